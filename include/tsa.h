@@ -341,6 +341,78 @@ int tsa_att_decode_static(const tsa_decode_cfg *cfg, const tsa_kv_seq *seqs, con
     int *statusWord, tsa_stream_t stream);
 size_t tsa_att_decode_static_capacity_bytes(void);
 
+/* ---- paged KV cache ---------------------------------------------------------------------------
+ * The cache of tsa_kv_append / tsa_att_decode in pages, for servers whose sequences grow and end at different times.  It has no
+ * counterpart in the reference (TAttentionVecHistory keeps one growing array per sequence, code/gpt/train/cpu_infer.cpp:397-410).
+ * A pool of page_count pages is shared by all sequences; a page holds page_size tokens of all key heads, head by head:
+ *   k, v                8-bit [page_count][kv_heads][page_size][D];   k_scale, v_scale  scale_dtype [page_count][kv_heads][page_size]
+ *   pos    int32 [page_count][kv_heads][page_size]  positions of the tokens, for caches that are evicted from (NULL: a token's
+ *                                                   position is its slot)
+ *   weight f32   [page_count][kv_heads][page_size]  attention weights that the tokens have gathered (NULL: not kept)
+ * all contiguous, in device memory, 16-byte aligned.  Slot t of sequence s is slot t % page_size of page pageTable[s][t / page_size]
+ * (int32 [nSeq][maxPages], device memory; entries behind a sequence's last page are not read).  ctxLens[s] (device) is the number of
+ * slots that the sequence fills; tokens[s] (device; NULL without pos) the number of tokens that it has seen, so that its newest token
+ * has position tokens[s] - 1 (ctxLens[s] - 1 without pos).
+ * A page number outside the pool, or a length beyond the table's or the caller's bound, sets a bit of the status word; the rows
+ * concerned are not stored, attended, chosen or moved, and nothing outside the buffers is touched. */
+typedef struct {
+    void *k;
+    void *v;
+    void *k_scale;
+    void *v_scale;
+    int *pos;
+    float *weight;
+    int page_count;
+    int page_size; /* 16, 32, 64, 128 or 256 */
+    int kv_heads;
+} tsa_paged_kv;
+
+typedef struct {
+    int head_dim;       /* 64 or 128 */
+    int kv_dtype;       /* TSA_I8 or TSA_E4M3: type of k, v and of the queries */
+    int scale_dtype;    /* TSA_F16 or TSA_F32: type of k_scale / v_scale */
+    int out_dtype;      /* TSA_F32, TSA_F16 or TSA_BF16 (decode) */
+    float qk_vec_scale; /* query scale when qScale is absent (decode) */
+} tsa_paged_cfg;
+
+/* Stores new rows behind what the sequences hold: kNew, vNew 8-bit [rows][kv_heads * D], kScaleNew, vScaleNew f32 [kv_heads][rows]
+ * (the planes that tsa_norm_rope_quant and tsa_matmul_norm_rope_quant write), rounded to the nearest scale_dtype.  Rows
+ * [rowStarts[s], rowStarts[s + 1]) (device int32 [nSeq + 1], ascending; NULL: one row per sequence) are sequence s's; ctxLens and
+ * tokens count them already, so the last of them goes to slot ctxLens[s] - 1 with position tokens[s] - 1.  Rows in front of
+ * rowStarts[0] or from rowStarts[nSeq] on are ignored.  Weights of the new slots become 0. */
+int tsa_paged_append(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens,
+    const int *rowStarts, int nSeq, int rows, tsa_ptr2d kNew, tsa_ptr2d kScaleNew, tsa_ptr2d vNew, tsa_ptr2d vScaleNew, int *statusWord,
+    tsa_stream_t stream);
+
+/* tsa_att_decode over the pages: each sequence's newest token attends to the keys with positions cur - window .. cur - 1, cur being its
+ * own (window 0: itself), with the same logits, sink and result.  headCount query heads share the kv_heads key heads evenly: query head
+ * h reads key head h / (headCount / kv_heads).  q 8-bit [nSeq][headCount * D] of kv_dtype, qScale f32 [nSeq][headCount] (may be
+ * absent), out [nSeq][headCount * D] of out_dtype.  Sequences without keys give zeros.
+ * A cache that keeps weights gets each attended key's weight, summed over the query heads of the key head, added to weight.
+ * maxCtx: host-side upper bound of ctxLens; it sizes the launch, and a sequence that turns out longer gives zeros and a bit of the
+ * status word.  Value scales below 2^-100 count as zero.  The same call gives the same bits every time.
+ * workspace: 16-byte aligned, not shared by calls in flight at the same time. */
+int tsa_paged_decode(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens, int nSeq,
+    int maxCtx, tsa_ptr2d q, tsa_ptr2d qScale, int window, float alibiSlope, tsa_ptr2d out, int headCount, void *workspace,
+    size_t workspaceBytes, int *statusWord, tsa_stream_t stream);
+size_t tsa_paged_decode_workspace_bytes(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, int nSeq, int headCount, int maxCtx);
+
+/* Which tokens stay when every sequence is cut to `keep` slots, for each key head by itself: the `recent` newest ones (positions above
+ * tokens[s] - 1 - recent) and, of the others, the heaviest by weight; among equals the lowest slot, NaN above all numbers.  Kept tokens
+ * behind slot `keep` move into the slots below it that became free, in the order of their slots:
+ *   moves      int32 [nSeq][kv_heads][moveCap][2]  (slot to write, slot to read), the rest (-1, -1)
+ *   moveCounts int32 [nSeq][kv_heads]
+ *   newLens    int32 [nSeq]                        min(ctxLens[s], keep)
+ * all device memory; moveCap at least min(keep, maxCtx - keep) and 1.  Sequences of up to `keep` slots have no moves.  Needs weight;
+ * of the cache only pos and weight are read (k, v and the scales may be NULL).  keep >= 1, 0 <= recent <= keep. */
+int tsa_paged_evict_select(const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens, int nSeq, int maxCtx, int keep,
+    int recent, int *moves, int moveCap, int *moveCounts, int *newLens, int *statusWord, tsa_stream_t stream);
+
+/* Carries the moves out: k, v, their scales, pos and weight of each slot to read go to the slot to write.  The slots that are written
+ * and those that are read have to be different ones, as above.  The sequences are then newLens long; pages behind that are free. */
+int tsa_paged_evict_move(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *moves, int moveCap,
+    const int *moveCounts, int nSeq, int *statusWord, tsa_stream_t stream);
+
 /* ---- host-side span preprocessing (CPU) ------------------------------------------------------
  * tsa_make_window_spans: causal window mask of AddAttSpans (code/gpt/att/sliding_window.cpp:80-87):
  *   row i of a fragment starting at f0 attends [max(f0, i - window), i - 1]; window <= 0: whole prefix.

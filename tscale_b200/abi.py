@@ -49,6 +49,17 @@ class DecodeCfg(ctypes.Structure):
     _fields_ = [("head_dim", c_int), ("scale_dtype", c_int), ("out_dtype", c_int), ("qk_vec_scale", c_float)]
 
 
+class PagedKv(ctypes.Structure):
+    """tsa_paged_kv"""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("pos", c_void_p), ("weight", c_void_p),
+                ("page_count", c_int), ("page_size", c_int), ("kv_heads", c_int)]
+
+
+class PagedCfg(ctypes.Structure):
+    """tsa_paged_cfg"""
+    _fields_ = [("head_dim", c_int), ("kv_dtype", c_int), ("scale_dtype", c_int), ("out_dtype", c_int), ("qk_vec_scale", c_float)]
+
+
 class InferDims(ctypes.Structure):
     """tsa_infer_dims"""
     _fields_ = [("dim", c_int), ("head_dim", c_int), ("head_count", c_int), ("relu_dim", c_int), ("vocab_size", c_int),
@@ -81,6 +92,7 @@ EXPORTS = [
     "tsa_att_fwd_to", "tsa_att_fwd_kv", "tsa_peer_scatter",
     "tsa_transpose_attention_device", "tsa_transpose_attention_device_workspace_bytes", "tsa_group_attention_device",
     "tsa_group_attention_device_workspace_bytes",
+    "tsa_paged_append", "tsa_paged_decode", "tsa_paged_decode_workspace_bytes", "tsa_paged_evict_select", "tsa_paged_evict_move",
 ]
 
 
@@ -138,6 +150,15 @@ def _declare(lib):
                                           P, c_int, c_void_p, c_void_p]
     lib.tsa_att_decode_static_capacity_bytes.restype = c_size_t
     lib.tsa_att_decode_static_capacity_bytes.argtypes = []
+    lib.tsa_paged_append.argtypes = [ctypes.POINTER(PagedCfg), ctypes.POINTER(PagedKv), P, c_void_p, c_void_p, c_void_p, c_int, c_int, P, P, P, P,
+                                     c_void_p, c_void_p]
+    lib.tsa_paged_decode.argtypes = [ctypes.POINTER(PagedCfg), ctypes.POINTER(PagedKv), P, c_void_p, c_void_p, c_int, c_int, P, P, c_int, c_float, P,
+                                     c_int, c_void_p, c_size_t, c_void_p, c_void_p]
+    lib.tsa_paged_decode_workspace_bytes.restype = c_size_t
+    lib.tsa_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(PagedCfg), ctypes.POINTER(PagedKv), c_int, c_int, c_int]
+    lib.tsa_paged_evict_select.argtypes = [ctypes.POINTER(PagedKv), P, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                                           c_void_p, c_void_p, c_void_p]
+    lib.tsa_paged_evict_move.argtypes = [ctypes.POINTER(PagedCfg), ctypes.POINTER(PagedKv), P, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]
     lib.tsa_matmul_norm_rope_quant.argtypes = [c_int, c_int, c_float, c_float, P, P, P, c_float, P, P, c_int, c_int, c_int, c_void_p, c_void_p]
     lib.tsa_infer_workspace_bytes.restype = c_size_t
     lib.tsa_infer_workspace_bytes.argtypes = [ctypes.POINTER(InferModel), c_int, c_int]

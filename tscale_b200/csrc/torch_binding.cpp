@@ -11,6 +11,7 @@
 #include <Python.h>
 #include <dlfcn.h>
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include "tsa.h"
@@ -34,6 +35,11 @@ struct TEntries {
     decltype(&tsa_att_decode_static) AttDecodeStatic;
     decltype(&tsa_att_decode_workspace_bytes) AttDecodeWs;
     decltype(&tsa_infer_step) InferStep;
+    decltype(&tsa_paged_append) PagedAppend;
+    decltype(&tsa_paged_decode) PagedDecode;
+    decltype(&tsa_paged_decode_workspace_bytes) PagedDecodeWs;
+    decltype(&tsa_paged_evict_select) PagedEvictSelect;
+    decltype(&tsa_paged_evict_move) PagedEvictMove;
 } g;
 
 PyObject *g_outOfMemory; // torch.OutOfMemoryError
@@ -235,6 +241,11 @@ PyObject *Bind(PyObject *, PyObject *const *a, Py_ssize_t n)
         get(g.AttDecodeStatic, "tsa_att_decode_static");
         get(g.AttDecodeWs, "tsa_att_decode_workspace_bytes");
         get(g.InferStep, "tsa_infer_step");
+        get(g.PagedAppend, "tsa_paged_append");
+        get(g.PagedDecode, "tsa_paged_decode");
+        get(g.PagedDecodeWs, "tsa_paged_decode_workspace_bytes");
+        get(g.PagedEvictSelect, "tsa_paged_evict_select");
+        get(g.PagedEvictMove, "tsa_paged_evict_move");
         Py_RETURN_NONE;
     });
 }
@@ -469,12 +480,208 @@ PyObject *InferStep(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 
+// ---- paged key-value cache: every tensor of a call is on one GPU, and the call runs on that GPU's current stream whatever GPU is current
+
+int Code8(const at::Tensor &t)
+{
+    switch (t.scalar_type()) {
+    case at::kChar:
+        return TSA_I8;
+    case at::kByte:
+    case at::kFloat8_e4m3fn:
+        return TSA_E4M3;
+    default:
+        return -1;
+    }
+}
+
+int Size(int64_t n)
+{
+    Need(n >= 0 && n <= 0x7fffffff, PyExc_AssertionError, "size beyond 32 bits");
+    return (int)n;
+}
+
+void SameGpu(const at::Tensor &first, std::initializer_list<const at::Tensor *> others)
+{
+    bool ok = first.is_cuda();
+    for (const at::Tensor *t : others) {
+        ok = ok && (!t || t->device() == first.device());
+    }
+    Need(ok, PyExc_AssertionError, "expected tensors of one GPU");
+}
+
+const at::Tensor *IntVector(PyObject *o, int64_t n)
+{
+    const at::Tensor *t = Tensor(o);
+    Need(!t || (t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() >= n), PyExc_AssertionError, "expected a contiguous int32 tensor with an entry per sequence");
+    return t;
+}
+
+// two-dimensional argument of a 32-bit type
+tsa_ptr2d Plane(const at::Tensor *t, at::ScalarType type, const char *text)
+{
+    Need(!t || t->scalar_type() == type, PyExc_AssertionError, text);
+    return P2D(t);
+}
+
+// (k, v, k_scale, v_scale, pos, weight), page table, ctxLens, tokens
+struct TPaged {
+    tsa_paged_kv Kv = {};
+    tsa_paged_cfg Cfg = {};
+    tsa_ptr2d Table;
+    const at::Tensor *Planes[6], *TableT, *Lens, *Tokens = nullptr;
+    int NSeq;
+    const int *LensPtr() const { return (const int *)Lens->data_ptr(); }
+    const int *TokensPtr() const { return Tokens ? (const int *)Tokens->data_ptr() : nullptr; }
+
+    TPaged(PyObject *kv, PyObject *table, PyObject *lens, PyObject *tokens, bool vectors)
+    {
+        Need(PyTuple_Check(kv) && PyTuple_GET_SIZE(kv) == 6, PyExc_TypeError, "expected a tuple (k, v, k_scale, v_scale, pos, weight)");
+        for (int i = 0; i < 6; ++i) {
+            Planes[i] = Tensor(PyTuple_GET_ITEM(kv, i));
+        }
+        const at::Tensor *k = Planes[0], *v = Planes[1], *ks = Planes[2], *vs = Planes[3], *shape = vectors ? ks : Planes[5];
+        Need(shape != nullptr && shape->dim() == 3, PyExc_AssertionError, "expected planes [pages][key heads][page size]");
+        for (int i = 2; i < 6; ++i) {
+            Need(!Planes[i] || (Planes[i]->sizes() == shape->sizes() && Planes[i]->is_contiguous()), PyExc_AssertionError,
+                "expected contiguous planes [pages][key heads][page size] of one shape");
+        }
+        Need((!Planes[4] || Planes[4]->scalar_type() == at::kInt) && (!Planes[5] || Planes[5]->scalar_type() == at::kFloat), PyExc_AssertionError,
+            "expected int32 positions and float32 weights");
+        if (vectors) {
+            Need(k && v && vs && k->dim() == 4 && k->sizes() == v->sizes() && k->is_contiguous() && v->is_contiguous() && k->sizes().slice(0, 3) == shape->sizes(),
+                PyExc_AssertionError, "expected contiguous k and v [pages][key heads][page size][head size] and their scales");
+            Need(Code8(*k) >= 0 && Code8(*k) == Code8(*v), PyExc_AssertionError, "expected k and v of one 8-bit type");
+            Need(ks->scalar_type() == vs->scalar_type() && (ks->scalar_type() == at::kHalf || ks->scalar_type() == at::kFloat), PyExc_AssertionError,
+                "expected float16 or float32 scales");
+            Cfg.head_dim = Size(k->size(3));
+            Cfg.kv_dtype = Code8(*k);
+            Cfg.scale_dtype = ks->scalar_type() == at::kHalf ? TSA_F16 : TSA_F32;
+            Kv.k = k->data_ptr();
+            Kv.v = v->data_ptr();
+            Kv.k_scale = ks->data_ptr();
+            Kv.v_scale = vs->data_ptr();
+        }
+        Kv.pos = Planes[4] ? (int *)Planes[4]->data_ptr() : nullptr;
+        Kv.weight = Planes[5] ? (float *)Planes[5]->data_ptr() : nullptr;
+        Kv.page_count = Size(shape->size(0));
+        Kv.kv_heads = Size(shape->size(1));
+        Kv.page_size = Size(shape->size(2));
+        TableT = &NeedTensor(table);
+        Table = Plane(TableT, at::kInt, "expected an int32 page table");
+        Lens = &NeedTensor(lens);
+        IntVector(lens, 0);
+        NSeq = Size(Lens->numel());
+        Tokens = IntVector(tokens, NSeq);
+    }
+    const at::Tensor &First() const { return *TableT; }
+    void OneGpu(std::initializer_list<const at::Tensor *> others) const
+    {
+        SameGpu(*TableT, {Planes[0], Planes[1], Planes[2], Planes[3], Planes[4], Planes[5], Lens, Tokens});
+        SameGpu(*TableT, others);
+    }
+    // same 8-bit type as the cache
+    tsa_ptr2d Codes(const at::Tensor &t) const
+    {
+        Need(Code8(t) == Cfg.kv_dtype, PyExc_AssertionError, "expected vectors of the cache's 8-bit type");
+        return P2D(t);
+    }
+};
+
+// kv, table, ctxLens, tokens, rowStarts, kNew, kScaleNew, vNew, vScaleNew, status
+PyObject *PagedAppend(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return Guard<10>(n, [&] {
+        const TPaged p(a[0], a[1], a[2], a[3], true);
+        const at::Tensor *starts = IntVector(a[4], p.NSeq + 1), *status = Tensor(a[9]);
+        const at::Tensor &k = NeedTensor(a[5]), &ks = NeedTensor(a[6]), &v = NeedTensor(a[7]), &vs = NeedTensor(a[8]);
+        const tsa_ptr2d k2 = p.Codes(k), v2 = p.Codes(v), ks2 = Plane(&ks, at::kFloat, "expected float32 scales of the new rows"),
+                        vs2 = Plane(&vs, at::kFloat, "expected float32 scales of the new rows");
+        p.OneGpu({starts, &k, &ks, &v, &vs, status});
+        const c10::cuda::CUDAGuard guard(p.First().device());
+        tsa_stream_t stream = Stream();
+        return PyLong_FromLong(Unlocked([&] {
+            return g.PagedAppend(&p.Cfg, &p.Kv, p.Table, p.LensPtr(), p.TokensPtr(), starts ? (const int *)starts->data_ptr() : nullptr, p.NSeq, k2.ysize, k2, ks2, v2, vs2,
+                status ? (int *)status->data_ptr() : nullptr, stream);
+        }));
+    });
+}
+
+// kv, table, ctxLens, tokens, maxCtx (None: what the table has room for), q, qScale, vecScale, window, slope, outDtype, out, workspace, status
+PyObject *PagedDecode(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return Guard<14>(n, [&] {
+        TPaged p(a[0], a[1], a[2], a[3], true);
+        const at::Tensor &q = NeedTensor(a[5]);
+        const at::Tensor *qs = Tensor(a[6]), *given = Tensor(a[11]), *ws = Tensor(a[12]), *status = Tensor(a[13]);
+        const tsa_ptr2d q2 = p.Codes(q), qs2 = Plane(qs, at::kFloat, "expected float32 query scales");
+        Need(p.Cfg.head_dim > 0 && q2.xsize % p.Cfg.head_dim == 0, PyExc_AssertionError, "expected queries [sequences][heads * head size]");
+        const int heads = q2.xsize / p.Cfg.head_dim, window = (int)Int(a[8]);
+        const int maxCtx = a[4] == Py_None ? Size((int64_t)p.Table.xsize * p.Kv.page_size) : (int)Int(a[4]);
+        const float slope = Float(a[9]);
+        p.Cfg.qk_vec_scale = Float(a[7]);
+        p.Cfg.out_dtype = given ? TsaType(*given) : (int)Int(a[10]);
+        p.OneGpu({&q, qs, given, ws, status});
+        const c10::cuda::CUDAGuard guard(p.First().device());
+        const at::Tensor out = given ? *given : Empty(p.NSeq, (int64_t)heads * p.Cfg.head_dim, TorchType(p.Cfg.out_dtype), q);
+        const tsa_ptr2d o2 = P2D(out);
+        const at::Tensor space = ws ? *ws : EmptyBytes(g.PagedDecodeWs(&p.Cfg, &p.Kv, p.NSeq, heads, maxCtx), q);
+        tsa_stream_t stream = Stream();
+        const int rc = Unlocked([&] {
+            return g.PagedDecode(&p.Cfg, &p.Kv, p.Table, p.LensPtr(), p.TokensPtr(), p.NSeq, maxCtx, q2, qs2, window, slope, o2, heads, space.data_ptr(),
+                (size_t)space.nbytes(), status ? (int *)status->data_ptr() : nullptr, stream);
+        });
+        return Result(rc, out);
+    });
+}
+
+// kv, table, ctxLens, tokens, maxCtx (None: what the table has room for), keep, recent, status
+PyObject *PagedEvictSelect(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return Guard<8>(n, [&] {
+        const TPaged p(a[0], a[1], a[2], a[3], false);
+        const at::Tensor *status = Tensor(a[7]);
+        const int maxCtx = a[4] == Py_None ? Size((int64_t)p.Table.xsize * p.Kv.page_size) : (int)Int(a[4]), keep = (int)Int(a[5]), recent = (int)Int(a[6]);
+        p.OneGpu({status});
+        const c10::cuda::CUDAGuard guard(p.First().device());
+        const int cap = std::max(1, std::min(keep, maxCtx - keep));
+        const at::TensorOptions ints = at::TensorOptions().dtype(at::kInt).device(p.First().device());
+        const at::Tensor moves = at::empty({p.NSeq, p.Kv.kv_heads, cap, 2}, ints), counts = at::empty({p.NSeq, p.Kv.kv_heads}, ints), lens = at::empty({p.NSeq}, ints);
+        tsa_stream_t stream = Stream();
+        const int rc = Unlocked([&] {
+            return g.PagedEvictSelect(&p.Kv, p.Table, p.LensPtr(), p.TokensPtr(), p.NSeq, maxCtx, keep, recent, (int *)moves.data_ptr(), cap, (int *)counts.data_ptr(),
+                (int *)lens.data_ptr(), status ? (int *)status->data_ptr() : nullptr, stream);
+        });
+        return Result(rc, moves, counts, lens);
+    });
+}
+
+// kv, table, moves, counts, status
+PyObject *PagedEvictMove(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return Guard<5>(n, [&] {
+        const at::Tensor &moves = NeedTensor(a[2]), *status = Tensor(a[4]);
+        const TPaged p(a[0], a[1], a[3], Py_None, true); // the counts in the place of the lengths
+        Need(moves.dim() == 4 && moves.scalar_type() == at::kInt && moves.is_contiguous() && moves.size(3) == 2 && moves.size(1) == p.Kv.kv_heads && p.Lens->dim() == 2 &&
+                p.Lens->size(0) == moves.size(0) && p.Lens->size(1) == moves.size(1),
+            PyExc_AssertionError, "expected int32 moves [sequences][key heads][most moves][2] and counts [sequences][key heads]");
+        const int nSeq = Size(moves.size(0)), cap = Size(moves.size(2));
+        p.OneGpu({&moves, status});
+        const c10::cuda::CUDAGuard guard(p.First().device());
+        tsa_stream_t stream = Stream();
+        return PyLong_FromLong(Unlocked([&] {
+            return g.PagedEvictMove(&p.Cfg, &p.Kv, p.Table, (const int *)moves.data_ptr(), cap, p.LensPtr(), nSeq, status ? (int *)status->data_ptr() : nullptr, stream);
+        }));
+    });
+}
+
 #define FAST(name, fn) {name, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FAST("bind", Bind), FAST("att_fwd", AttFwd), FAST("att_bwd", AttBwd), FAST("quant_rows", QuantRows),
     FAST("norm_rope_quant", NormRopeQuant), FAST("matmul_norm_rope_quant", MatmulNormRopeQuant), FAST("rope_norm_bwd", RopeNormBwd),
     FAST("kv_product", KvProduct), FAST("kv_product_bwd", KvProductBwd), FAST("calc_dscale", CalcDScale), FAST("kv_append", KvAppend),
     FAST("att_decode_workspace_bytes", AttDecodeWorkspaceBytes),
-    FAST("att_decode", AttDecode), FAST("infer_step", InferStep), {nullptr, nullptr, 0, nullptr}};
+    FAST("att_decode", AttDecode), FAST("infer_step", InferStep), FAST("paged_append", PagedAppend), FAST("paged_decode", PagedDecode),
+    FAST("paged_evict_select", PagedEvictSelect), FAST("paged_evict_move", PagedEvictMove), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "torch-tensor binding of libtsa_b200.so", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 } // namespace

@@ -5,6 +5,7 @@ qk = queries, qv = keys, v = values, per-head scale planes [H][len], grouped spa
 Everything runs on the GPU through libtsa_b200.so; torch only owns the memory and the stream.  The calls a step runs through
 go by way of the compiled binding (_native.so, csrc/torch_binding.cpp); the rest uses ctypes.
 """
+import collections
 import ctypes
 
 import numpy as np
@@ -351,3 +352,127 @@ class KVCache:
                                      None, status)
         check(rc)
         return out
+
+
+PagedKV = collections.namedtuple("PagedKV", "k v k_scale v_scale pos weight", defaults=(None, None))
+PagedKV.__doc__ = """Pools of a paged KV cache (tsa_paged_kv), all contiguous: k, v [pages][key heads][page size][head size], int8 or e4m3
+(torch.float8_e4m3fn, or its bytes as uint8); k_scale, v_scale [pages][key heads][page size], float16 or float32; pos int32 and weight
+float32 of the same shape, or None.  Token t of sequence s is in slot t % page size of page page_table[s][t // page size].  The paged_
+functions take any tuple of these six."""
+
+
+def paged_append(kv, page_table, ctx_lens, k, k_scale, v, v_scale, row_starts=None, tokens=None, status=None):
+    """Stores new rows behind what the sequences hold (tsa_paged_append): k, v 8-bit [rows][key heads * head size], k_scale, v_scale float32
+    [key heads][rows].  row_starts int32 [sequences + 1]: sequence s has rows row_starts[s] .. row_starts[s + 1] - 1; None: one row per
+    sequence.  ctx_lens and tokens count the new rows already."""
+    check(_native.paged_append(kv, page_table, ctx_lens, tokens, row_starts, k, k_scale, v, v_scale, status))
+
+
+def paged_decode(kv, page_table, ctx_lens, q, q_scale, window, slope, max_ctx=None, out_dtype=torch.float32, tokens=None, vec_scale=1.0, out=None,
+                 workspace=None, status=None):
+    """Attention of each sequence's newest token over the pages (tsa_paged_decode): q [sequences][heads * head size] in the cache's type,
+    q_scale float32 [sequences][heads] or None (vec_scale for all).  Query heads share the key heads evenly.  max_ctx: bound of ctx_lens
+    (None: what the page table has room for).  A cache with weights gets the attention weights added.  Returns out."""
+    rc, out = _native.paged_decode(kv, page_table, ctx_lens, tokens, max_ctx, q, q_scale, vec_scale, window, slope, _DT[out_dtype], out, workspace, status)
+    check(rc)
+    return out
+
+
+def paged_evict_select(kv, page_table, ctx_lens, keep, recent, max_ctx=None, tokens=None, status=None):
+    """Which tokens stay when every sequence is cut to `keep` slots (tsa_paged_evict_select): the `recent` newest and the heaviest others, for
+    each key head.  Returns (moves int32 [sequences][key heads][most][2], counts int32 [sequences][key heads], new lengths int32 [sequences])."""
+    rc, moves, counts, lens = _native.paged_evict_select(kv, page_table, ctx_lens, tokens, max_ctx, keep, recent, status)
+    check(rc)
+    return moves, counts, lens
+
+
+def paged_evict_move(kv, page_table, moves, counts, status=None):
+    """Carries the moves of paged_evict_select out (tsa_paged_evict_move)."""
+    check(_native.paged_evict_move(kv, page_table, moves, counts, status))
+
+
+class PagedKVCache:
+    """KV cache of n_seq sequences in a pool of page_count pages, with the book-keeping on the host: which pages are free, how many tokens each
+    sequence holds.  max_pages: pages that one sequence can have (default: all).  evict: the cache keeps positions and weights, so that
+    `evict` can cut it.  The device tensors page_table, ctx_lens and tokens keep their addresses, so captured calls can be replayed after
+    `extend` and `evict` (decode then needs a max_ctx that covers the replays).  Calls on one cache are ordered by one stream."""
+
+    def __init__(self, n_seq, page_count, kv_heads, head_dim, device, page_size=64, max_pages=None, kv_dtype="i8", scale_dtype=torch.float16,
+                 out_dtype=torch.float32, qk_vec_scale=1.0, evict=False):
+        max_pages = page_count if max_pages is None else max_pages
+        if min(n_seq, page_count, kv_heads, page_size, max_pages) < 1 or kv_dtype not in ("i8", "e4m3"):
+            raise ValueError("PagedKVCache: sizes must be positive and kv_dtype 'i8' or 'e4m3'")
+        self.n_seq, self.page_count, self.page_size, self.max_pages = n_seq, page_count, page_size, max_pages
+        self.kv_heads, self.head_dim, self.out_dtype, self.qk_vec_scale = kv_heads, head_dim, out_dtype, qk_vec_scale
+        plane = (page_count, kv_heads, page_size)
+        codes = torch.int8 if kv_dtype == "i8" else torch.float8_e4m3fn
+        vec = lambda: torch.zeros(plane + (head_dim,), dtype=torch.int8, device=device).view(codes)  # noqa: E731
+        own = lambda dt: torch.zeros(plane, dtype=dt, device=device)  # noqa: E731
+        self.kv = PagedKV(vec(), vec(), own(scale_dtype), own(scale_dtype), own(torch.int32) if evict else None, own(torch.float32) if evict else None)
+        # table, lengths and token counts in one array, so that one copy brings a change of them to the device
+        self._host = np.full(n_seq * (max_pages + 2), -1, dtype=np.int32)
+        self._host[n_seq * max_pages:] = 0
+        self._dev = torch.from_numpy(self._host.copy()).to(device)
+        self._table = self._host[:n_seq * max_pages].reshape(n_seq, max_pages)
+        self.lens, self.seen = self._host[n_seq * max_pages:].reshape(2, n_seq)  # slots filled, tokens seen
+        self.page_table = self._dev[:n_seq * max_pages].view(n_seq, max_pages)
+        self.ctx_lens = self._dev[n_seq * max_pages:n_seq * (max_pages + 1)]
+        self.tokens = self._dev[n_seq * (max_pages + 1):] if evict else None
+        self.free = list(range(page_count - 1, -1, -1))
+
+    def _upload(self):
+        host = torch.from_numpy(self._host.copy())
+        self._dev.copy_(host.pin_memory() if self._dev.is_cuda else host, non_blocking=True)
+
+    def _pages(self, slots):
+        return -(-int(slots) // self.page_size)
+
+    def extend(self, counts=1):
+        """Makes room for counts[s] new tokens of each sequence (one number: the same for all), which the next `append` stores.  Returns the
+        row_starts of that append; None where every sequence gets one row.  Raises TsaError, and changes nothing, if the pages do not suffice."""
+        counts = np.broadcast_to(np.asarray(counts, dtype=np.int64), (self.n_seq,))
+        if (counts < 0).any():
+            raise abi.TsaError(abi.TSA_BAD_ARG, "PagedKVCache.extend: negative count")
+        after = self.lens + counts
+        need = [self._pages(b) - self._pages(a) for a, b in zip(self.lens, after)]
+        if max(self._pages(n) for n in after) > self.max_pages or sum(need) > len(self.free):
+            raise abi.TsaError(abi.TSA_BAD_ARG, "PagedKVCache.extend: %d pages needed, %d free; a sequence has at most %d"
+                               % (sum(need), len(self.free), self.max_pages))
+        for s, n in enumerate(need):
+            have = self._pages(self.lens[s])
+            for i in range(n):
+                self._table[s, have + i] = self.free.pop()
+        self.lens += counts.astype(np.int32)
+        self.seen += counts.astype(np.int32)
+        self._upload()
+        if (counts == 1).all():
+            return None
+        return torch.from_numpy(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)).to(self._dev.device)
+
+    def append(self, k, k_scale, v, v_scale, row_starts=None, status=None):
+        paged_append(self.kv, self.page_table, self.ctx_lens, k, k_scale, v, v_scale, row_starts, self.tokens, status)
+
+    def decode(self, q, q_scale, window, slope, max_ctx=None, out=None, status=None):
+        """max_ctx: None: the longest sequence of now."""
+        return paged_decode(self.kv, self.page_table, self.ctx_lens, q, q_scale, window, slope, int(self.lens.max()) if max_ctx is None else max_ctx,
+                            self.out_dtype, self.tokens, self.qk_vec_scale, out, None, status)
+
+    def evict(self, keep, recent=1, status=None):
+        """Cuts every sequence to `keep` slots: for each key head the `recent` newest tokens and the heaviest others stay.  Frees their pages."""
+        moves, counts, _ = paged_evict_select(self.kv, self.page_table, self.ctx_lens, keep, recent, int(self.lens.max()), self.tokens, status)
+        paged_evict_move(self.kv, self.page_table, moves, counts, status)
+        for s in range(self.n_seq):
+            self._cut(s, min(int(self.lens[s]), keep))
+        self._upload()
+
+    def release(self, seq):
+        """The sequence's pages become free, and it is empty."""
+        self._cut(seq, 0)
+        self.seen[seq] = 0
+        self._upload()
+
+    def _cut(self, seq, slots):
+        for i in range(self._pages(slots), self._pages(self.lens[seq])):
+            self.free.append(int(self._table[seq, i]))
+            self._table[seq, i] = -1
+        self.lens[seq] = slots
