@@ -158,14 +158,19 @@ struct TSelectParams {
     const int *CtxLens, *Tokens;
     int NSeq, Keep, Recent, MoveCap;
     int MaxCtx; // the caller's bound of CtxLens
+    int Cluster; // CTAs per key head of a sequence
     int2 *Moves; // [nSeq][kvHeads][MoveCap]
     int *Counts; // [nSeq][kvHeads]
     int *NewLens;
     int *Status;
 };
 
-constexpr int SEL_THREADS = 1024;
+constexpr int SEL_THREADS = 512;
 constexpr int SEL_WARPS = SEL_THREADS / 32;
+constexpr int SEL_BINS = 2048;            // 11, 11 and 10 bits of the order
+constexpr int SEL_MAX_CLUSTER = 8;
+constexpr int SEL_SLOTS = 4096;           // slots of a CTA where there are CTAs enough
+constexpr int SEL_MAX_SLICE = 48 * 1024;  // slots whose orders fit shared memory
 
 // weights as unsigned integers of the same order; -0 counts as 0, NaN as the greatest; tokens that stay whatever their weight are above all
 constexpr unsigned SEL_PINNED = 0xffffffffu, SEL_NAN = 0xfffffffeu;
@@ -175,47 +180,77 @@ __device__ __forceinline__ unsigned WeightOrder(float w)
     return w != w ? SEL_NAN : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-__device__ __forceinline__ unsigned SlotOrder(const TSelectParams &p, const int *table, int head, int slot, int newest, int *bad)
+// orders of slots slot .. slot + 3 (slot a multiple of 4); slots of pages outside the pool are the lightest
+__device__ __forceinline__ uint4 SlotOrders(const TSelectParams &p, const int *table, int head, int slot, int newest, bool *bad)
 {
     const TPages &c = p.C;
     const int page = table[slot >> c.PageShift];
-    if (page < 0 || page >= c.PageCount) {
-        *bad = 1;
-        return 0;
+    if ((unsigned)page >= (unsigned)c.PageCount) {
+        *bad = true;
+        return make_uint4(0, 0, 0, 0);
     }
     const size_t at = PlaneSlot(c, page, head) + (slot & ((1 << c.PageShift) - 1));
-    const int pos = c.Pos ? c.Pos[at] : slot;
-    return pos > newest - p.Recent ? SEL_PINNED : WeightOrder(c.Weight[at]);
-}
-
-// sum over the block of each thread's value; every thread gets it
-__device__ __forceinline__ int BlockSum(int v, int *red)
-{
-    v = __reduce_add_sync(0xffffffffu, v);
-    __syncthreads(); // the previous sums have been read
-    if ((threadIdx.x & 31) == 0) {
-        red[threadIdx.x >> 5] = v;
+    const float4 w = *reinterpret_cast<const float4 *>(c.Weight + at);
+    uint4 o = make_uint4(WeightOrder(w.x), WeightOrder(w.y), WeightOrder(w.z), WeightOrder(w.w));
+    if (p.Recent > 0) {
+        const int4 pos = c.Pos ? *reinterpret_cast<const int4 *>(c.Pos + at) : make_int4(slot, slot + 1, slot + 2, slot + 3);
+        const int old = newest - p.Recent;
+        o.x = pos.x > old ? SEL_PINNED : o.x;
+        o.y = pos.y > old ? SEL_PINNED : o.y;
+        o.z = pos.z > old ? SEL_PINNED : o.z;
+        o.w = pos.w > old ? SEL_PINNED : o.w;
     }
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, red[threadIdx.x & 31]);
+    return o;
 }
 
-// One CTA per (sequence, key head).  Each warp owns a contiguous run of slots, so that ranks in slot order are a warp's ballots on top of
-// the sums of the warps before it.  The keep-th largest weight is found bit by bit from the top (32 counts).
+__device__ __forceinline__ void ClusterSync()
+{
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// word of another CTA of the cluster at the place of `mine` in its shared memory
+__device__ __forceinline__ unsigned ClusterAddress(const void *mine, int rank)
+{
+    unsigned r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((unsigned)__cvta_generic_to_shared(mine)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ uint4 ClusterLoad16(unsigned address)
+{
+    uint4 r;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(address) : "memory");
+    return r;
+}
+
+struct TSelectShared {
+    unsigned Hist[3][SEL_BINS];
+    int WarpSum[SEL_WARPS];
+    int Found[2];            // bin, and how many are still to be taken from it
+    int4 Total;              // of this CTA: ties, holes, movers
+    int4 WarpOf[SEL_WARPS];
+};
+
+// One cluster of CTAs per (sequence, key head); CTA `rank` has the slots [rank * slice, (rank + 1) * slice), each warp a contiguous run of
+// them, four to a lane.  The keep-th largest order is found in three digits: counts of the digit among the orders that agree in the digits
+// before (shared memory, the CTAs' counts added through distributed shared memory), then the sum from the top.  Ranks in slot order are
+// ballots on top of the sums of the warps and CTAs before.  CACHED: the orders stay in shared memory after they are read once.
+template <bool CACHED>
 __global__ void __launch_bounds__(SEL_THREADS) PagedSelectKernel(const TSelectParams p)
 {
-    __shared__ int red[32];
-    __shared__ int holesOf[32], moversOf[32], tiesOf[32];
-    const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    PdlTrigger();
-    PdlWait();
+    extern __shared__ uint4 cached[];
+    __shared__ __align__(16) TSelectShared sh;
+    const int head = blockIdx.x / p.Cluster, rank = blockIdx.x % p.Cluster, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const TPages &c = p.C;
+    for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) {
+        sh.Hist[0][i] = 0;
+    }
+    PdlWait();
+    PdlTrigger();
     const int len = p.CtxLens[seq];
     const size_t unit = (size_t)seq * c.KvHeads + head;
     int2 *moves = p.Moves + unit * p.MoveCap;
     const bool tooLong = len > p.MaxCtx || len > TableTokens(c);
     const bool none = len <= p.Keep || tooLong;
-    if (tid == 0) {
+    if (tid == 0 && rank == 0) {
         if (tooLong && p.Status) {
             atomicOr(p.Status, kDevBadSpan);
         }
@@ -226,89 +261,245 @@ __global__ void __launch_bounds__(SEL_THREADS) PagedSelectKernel(const TSelectPa
             p.Counts[unit] = 0;
         }
     }
-    if (none) {
-        for (int i = tid; i < p.MoveCap; i += SEL_THREADS) {
+    if (none) { // the same in all CTAs of the cluster
+        for (int i = rank * SEL_THREADS + tid; i < p.MoveCap; i += p.Cluster * SEL_THREADS) {
             moves[i] = make_int2(-1, -1);
         }
         return;
     }
     const int *table = c.Table.Row(seq);
     const int newest = (p.Tokens ? p.Tokens[seq] : len) - 1;
-    const int per = ((len + SEL_WARPS - 1) / SEL_WARPS + 31) & ~31; // slots of a warp
-    const int beg = min(warp * per, len), end = min(beg + per, len);
-    int bad = 0;
-    unsigned cut = 0; // largest value that at least Keep slots reach
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned probe = cut | (1u << bit);
-        int n = 0;
-        for (int s = beg + lane; s < end; s += 32) {
-            n += SlotOrder(p, table, head, s, newest, &bad) >= probe;
+    // slots of a CTA and of a warp: equal parts of what the sequence has, in whole steps of 128
+    const int warps = p.Cluster * SEL_WARPS;
+    const int per = ((len + warps - 1) / warps + 127) & ~127;
+    const int slice = per * SEL_WARPS;
+    const int beg = min(rank * slice + warp * per, len), end = min(beg + per, len);
+    bool bad = false;
+    auto orders = [&](int s) { return CACHED ? cached[(s - rank * slice) >> 2] : SlotOrders(p, table, head, s, newest, &bad); };
+    auto count = [&](unsigned *hist, unsigned bin, bool in) {
+        // equal bins of a whole warp (weights that are all zero) are one addition
+        const unsigned first = __shfl_sync(0xffffffffu, bin, 0);
+        if (__all_sync(0xffffffffu, in && bin == first)) {
+            if (lane == 0) {
+                atomicAdd(hist + bin, 32);
+            }
+        } else if (in) {
+            atomicAdd(hist + bin, 1);
         }
-        if (BlockSum(n, red) >= p.Keep) {
-            cut = probe;
+    };
+    __syncthreads(); // the counts are zero
+#pragma unroll 2
+    for (int s0 = beg; s0 < end; s0 += 128) {
+        const int s = s0 + 4 * lane;
+        uint4 o = make_uint4(0, 0, 0, 0);
+        if (s < end) {
+            o = SlotOrders(p, table, head, s, newest, &bad);
+            if (CACHED) {
+                cached[(s - rank * slice) >> 2] = o;
+            }
         }
+        count(sh.Hist[0], o.x >> 21, s < end);
+        count(sh.Hist[0], o.y >> 21, s + 1 < end);
+        count(sh.Hist[0], o.z >> 21, s + 2 < end);
+        count(sh.Hist[0], o.w >> 21, s + 3 < end);
     }
-    int above = 0, equal = 0;
-    for (int s = beg + lane; s < end; s += 32) {
-        const unsigned o = SlotOrder(p, table, head, s, newest, &bad);
-        above += o > cut;
-        equal += o == cut;
-    }
-    equal = __reduce_add_sync(0xffffffffu, equal);
-    if (lane == 0) {
-        tiesOf[warp] = equal;
-    }
-    int take = p.Keep - BlockSum(above, red); // of the slots at the border, the first `take`
-    for (int w = 0; w < warp; ++w) {
-        take -= tiesOf[w];
-    }
-    // two sweeps: count, then write
-    int hole = 0, mover = 0;
-    for (int sweep = 0; sweep < 2; ++sweep) {
-        int left = take;
-        for (int s0 = beg; s0 < end; s0 += 32) {
-            const int s = s0 + lane;
-            const unsigned o = s < end ? SlotOrder(p, table, head, s, newest, &bad) : 0;
-            const unsigned tie = __ballot_sync(0xffffffffu, s < end && o == cut);
-            const bool kept = s < end && (o > cut || (o == cut && __popc(tie & ((1u << lane) - 1)) < left));
-            left -= __popc(tie);
-            const bool isHole = s < end && !kept && s < p.Keep, isMover = kept && s >= p.Keep;
-            const unsigned hb = __ballot_sync(0xffffffffu, isHole), mb = __ballot_sync(0xffffffffu, isMover);
-            if (sweep) {
-                const int hr = hole + __popc(hb & ((1u << lane) - 1)), mr = mover + __popc(mb & ((1u << lane) - 1));
-                if (isHole && hr < p.MoveCap) {
-                    moves[hr].x = s;
-                }
-                if (isMover && mr < p.MoveCap) {
-                    moves[mr].y = s;
+    unsigned cut = 0;     // the digits found so far
+    int take = p.Keep;    // how many of the orders that agree with them stay
+#pragma unroll
+    for (int digit = 0; digit < 3; ++digit) {
+        constexpr int SHIFT[3] = {21, 10, 0};
+        const int bits = digit == 2 ? 10 : 11;
+        if (digit > 0) {
+            const unsigned mask = digit == 1 ? 0xffe00000u : 0xfffffc00u;
+            for (int s0 = beg; s0 < end; s0 += 128) {
+                const int s = s0 + 4 * lane;
+                const uint4 o = s < end ? orders(s) : make_uint4(0, 0, 0, 0);
+                const unsigned low = (1u << bits) - 1;
+                const bool x = s < end && (o.x & mask) == cut, y = s + 1 < end && (o.y & mask) == cut;
+                const bool z = s + 2 < end && (o.z & mask) == cut, w = s + 3 < end && (o.w & mask) == cut;
+                if (__any_sync(0xffffffffu, x | y | z | w)) {
+                    count(sh.Hist[digit], o.x >> SHIFT[digit] & low, x);
+                    count(sh.Hist[digit], o.y >> SHIFT[digit] & low, y);
+                    count(sh.Hist[digit], o.z >> SHIFT[digit] & low, z);
+                    count(sh.Hist[digit], o.w >> SHIFT[digit] & low, w);
                 }
             }
-            hole += __popc(hb);
-            mover += __popc(mb);
+        }
+        if (p.Cluster > 1) {
+            ClusterSync();
+        } else {
+            __syncthreads();
+        }
+        // thread t has bins [top - 4 t - 3, top - 4 t]: sums run from the largest bin down
+        const int first = (1 << 11) - 4 - 4 * tid; // digits of 10 bits use the lower half, the rest is zero
+        uint4 h = *reinterpret_cast<const uint4 *>(&sh.Hist[digit][first]);
+        for (int r = 1; r < p.Cluster; ++r) {
+            const uint4 o = ClusterLoad16(ClusterAddress(&sh.Hist[digit][first], (rank + r) % p.Cluster));
+            h.x += o.x;
+            h.y += o.y;
+            h.z += o.z;
+            h.w += o.w;
+        }
+        const int mine = (int)(h.x + h.y + h.z + h.w);
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            sum += lane >= o ? v : 0;
+        }
+        if (lane == 31) {
+            sh.WarpSum[warp] = sum;
+        }
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) {
+            sum += sh.WarpSum[w];
+        }
+        int above = sum - mine; // orders in larger bins
+        if (above < take && sum >= take) {
+            const unsigned b[4] = {h.w, h.z, h.y, h.x};
+            int i = 0;
+            while (above + (int)b[i] < take) {
+                above += b[i++];
+            }
+            sh.Found[0] = first + 3 - i;
+            sh.Found[1] = take - above;
+            sh.Total.w = b[i]; // how many agree
+        }
+        __syncthreads();
+        cut |= (unsigned)sh.Found[0] << SHIFT[digit];
+        take = sh.Found[1];
+    }
+    // `take` of the orders equal to cut stay, the first ones in slot order; mostly that is all of them
+    const bool allTies = sh.Total.w == take;
+    int ties = take;
+    if (!allTies) {
+        int n = 0;
+        for (int s0 = beg; s0 < end; s0 += 128) {
+            const int s = s0 + 4 * lane;
+            if (s < end) {
+                const uint4 o = orders(s);
+                n += (o.x == cut) + (s + 1 < end && o.y == cut) + (s + 2 < end && o.z == cut) + (s + 3 < end && o.w == cut);
+            }
+        }
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (lane == 0) {
+            sh.WarpOf[warp].x = n;
+        }
+        __syncthreads();
+        int before = 0, total = 0;
+        for (int w = 0; w < SEL_WARPS; ++w) {
+            before += w < warp ? sh.WarpOf[w].x : 0;
+            total += sh.WarpOf[w].x;
+        }
+        if (p.Cluster > 1) {
+            if (tid == 0) {
+                sh.Total.x = total;
+            }
+            ClusterSync();
+            for (int r = 0; r < rank; ++r) {
+                before += (int)ClusterLoad16(ClusterAddress(&sh.Total, r)).x;
+            }
+        }
+        ties -= before; // left for this warp's slots
+    }
+    // two sweeps: count, then write
+    int hole = 0, mover = 0, moved = 0;
+#pragma unroll
+    for (int sweep = 0; sweep < 2; ++sweep) {
+        int left = ties;
+        for (int s0 = beg; s0 < end; s0 += 128) {
+            const int s = s0 + 4 * lane;
+            const uint4 o4 = s < end ? orders(s) : make_uint4(0, 0, 0, 0);
+            const unsigned o[4] = {o4.x, o4.y, o4.z, o4.w};
+            const unsigned below = (1u << lane) - 1;
+            bool keep[4];
+            if (allTies) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    keep[i] = s + i < end && o[i] >= cut;
+                }
+            } else {
+                unsigned tie[4];
+                int before = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    tie[i] = __ballot_sync(0xffffffffu, s + i < end && o[i] == cut);
+                    before += __popc(tie[i] & below);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool mine = tie[i] >> lane & 1;
+                    keep[i] = s + i < end && (o[i] > cut || (mine && before < left));
+                    before += mine;
+                }
+                left -= __popc(tie[0]) + __popc(tie[1]) + __popc(tie[2]) + __popc(tie[3]);
+            }
+            int hb = 0, mb = 0, hn = 0, mn = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned h = __ballot_sync(0xffffffffu, s + i < end && !keep[i] && s + i < p.Keep);
+                const unsigned m = __ballot_sync(0xffffffffu, keep[i] && s + i >= p.Keep);
+                hb += __popc(h & below);
+                mb += __popc(m & below);
+                hn += __popc(h);
+                mn += __popc(m);
+            }
+            if (sweep) {
+                int hr = hole + hb, mr = mover + mb;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (s + i < end && !keep[i] && s + i < p.Keep && hr < p.MoveCap) {
+                        moves[hr++].x = s + i;
+                    }
+                    if (keep[i] && s + i >= p.Keep && mr < p.MoveCap) {
+                        moves[mr++].y = s + i;
+                    }
+                }
+            }
+            hole += hn;
+            mover += mn;
         }
         if (!sweep) {
             if (lane == 0) {
-                holesOf[warp] = hole;
-                moversOf[warp] = mover;
+                sh.WarpOf[warp] = make_int4(0, hole, mover, 0);
             }
             __syncthreads();
-            int total = 0;
+            int4 total = make_int4(0, 0, 0, 0);
             hole = mover = 0;
             for (int w = 0; w < SEL_WARPS; ++w) {
-                hole += w < warp ? holesOf[w] : 0;
-                mover += w < warp ? moversOf[w] : 0;
-                total += moversOf[w];
+                const int4 x = sh.WarpOf[w];
+                hole += w < warp ? x.y : 0;
+                mover += w < warp ? x.z : 0;
+                total.y += x.y;
+                total.z += x.z;
             }
-            for (int i = total + tid; i < p.MoveCap; i += SEL_THREADS) {
+            moved = total.z;
+            if (p.Cluster > 1) {
+                ClusterSync(); // the ties of Total have been read
+                if (tid == 0) {
+                    sh.Total = total;
+                }
+                ClusterSync();
+                for (int r = 0; r < p.Cluster; ++r) {
+                    const uint4 x = ClusterLoad16(ClusterAddress(&sh.Total, r));
+                    hole += r < rank ? (int)x.y : 0;
+                    mover += r < rank ? (int)x.z : 0;
+                    moved += r != rank ? (int)x.z : 0;
+                }
+            }
+            for (int i = moved + rank * SEL_THREADS + tid; i < p.MoveCap; i += p.Cluster * SEL_THREADS) {
                 moves[i] = make_int2(-1, -1);
             }
-            if (tid == 0) {
-                p.Counts[unit] = min(total, p.MoveCap);
+            if (tid == 0 && rank == 0) {
+                p.Counts[unit] = min(moved, p.MoveCap);
             }
         }
     }
     if (bad && p.Status) {
         atomicOr(p.Status, kDevBadSpan);
+    }
+    if (p.Cluster > 1) {
+        ClusterSync(); // no CTA leaves while another reads its shared memory
     }
 }
 
@@ -468,8 +659,34 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_evict_select(con
     p.Counts = moveCounts;
     p.NewLens = newLens;
     p.Status = statusWord;
+    const long long room = TableTokens(p.C);
+    const int longest = room < maxCtx ? (int)room : maxCtx;
+    int dev = 0, sms = 0;
+    rc = CheckCuda(cudaGetDevice(&dev), "cudaGetDevice");
+    if (rc == TSA_OK) {
+        rc = CheckCuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+    }
+    if (rc != TSA_OK) {
+        return rc;
+    }
+    // CTAs of SEL_SLOTS slots while all of them are resident at once (four to an SM)
+    p.Cluster = 1;
+    while (p.Cluster < SEL_MAX_CLUSTER && longest > SEL_SLOTS * p.Cluster && 2ll * p.Cluster * kv->kv_heads * nSeq <= 4ll * sms) {
+        p.Cluster *= 2;
+    }
+    const int warps = p.Cluster * SEL_WARPS;
+    const int slice = ((longest + warps - 1) / warps + 127) / 128 * 128 * SEL_WARPS;
+    const bool cached = slice <= SEL_MAX_SLICE;
+    const void *kern = cached ? (const void *)PagedSelectKernel<true> : (const void *)PagedSelectKernel<false>;
+    const size_t smem = cached ? (size_t)slice * sizeof(unsigned) : 0;
+    if (smem > 16 * 1024) { // beyond 48 KB with the counts
+        rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_SLICE * sizeof(unsigned)), "cudaFuncSetAttribute");
+        if (rc != TSA_OK) {
+            return rc;
+        }
+    }
     void *args[] = {&p};
-    return CheckCuda(LaunchPdl((const void *)PagedSelectKernel, dim3(kv->kv_heads, nSeq), dim3(SEL_THREADS), 0, (cudaStream_t)stream, args),
+    return CheckCuda(LaunchPdl(kern, dim3(kv->kv_heads * p.Cluster, nSeq), dim3(SEL_THREADS), smem, (cudaStream_t)stream, args, p.Cluster),
         "tsa_paged_evict_select launch");
 }
 
