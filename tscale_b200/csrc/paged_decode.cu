@@ -5,13 +5,12 @@
 //   weight_j += sum over the heads that share the key head of 2^z_j / (1 + sum)   (caches that keep weights)
 //
 // The stream of the cache bounds it: 2 D bytes of codes and two scales per key and key head, each read once.  The products run on the
-// warp's matrix instructions with the query heads of a key head as the 16 rows of A, so that up to 16 of them share what was loaded; with
-// up to eight the other eight rows carry the low parts of the weights (below).  Fragments come straight from global memory: the columns of
-// a tile of 16 keys and the order of the head's dimensions are free, and are taken such that every lane loads 16 bytes at a time, of
+// warp's matrix instructions, scores = q K^T with the query heads of a key head as rows and result^T = V^T weights^T with them as columns,
+// so that up to 16 heads share what was loaded.  Fragments come straight from global memory: the order of the keys in a tile of 16 and of
+// the head's dimensions are free, and are taken such that every lane loads 16 bytes at a time (lane = 4 g + t), of
 //   K: key 4 (g / 2) + 2 n + g % 2 for column g of score block n, dimensions 16 t .. 16 t + 15 (and 64 more)
-//   V: keys 4 t .. 4 t + 3, dimensions D / 8 g ..                                  (lane = 4 g + t)
-// which leaves lane (g, t) with the scores of head g for keys 4 t .. 4 t + 3: just the rows of V that it holds, so the weights are the A
-// fragment of the second product as they are.
+//   V: keys 4 t .. 4 t + 3, dimensions D / 8 g .. D / 8 g + D / 8 - 1
+// which leaves lane (g, t) with the scores of head g for keys 4 t .. 4 t + 3: the weights are the second product's B fragment as they are.
 //
 // Weights: 2^(z - ref) * vScale in two f16 parts (22 bits; 2^-25 of the largest at worst), ref being the running maximum of
 // z + log2 |vScale|, raised when a tile exceeds it by 2^8.  int8 products are exact in int32; e4m3 codes are exact in f16 and their
@@ -193,15 +192,16 @@ struct TScales<false> {
     __device__ __forceinline__ float Get(int i) const { return __uint_as_float(i == 0 ? X.x : i == 1 ? X.y : i == 2 ? X.z : X.w); }
 };
 
-// WIDE: more than eight query heads share a key head (all 16 rows are heads; otherwise rows 8 .. 15 carry the weights' low parts).
+// WIDE: more than eight query heads share a key head (otherwise rows 8 .. 15 of the scores are unused, and half the sums).
 // SINGLE: a CTA has one whole unit (short contexts): no ranges, no partial sums, no second kernel.
 template <int D, bool E4M3, bool SCALE_F16, bool WIDE, bool TRACK, bool SINGLE>
-__global__ void __launch_bounds__(PD_THREADS, D == 128 ? 3 : 5) PagedDecodeKernel(const TPagedDecodeParams p)
+__global__ void __launch_bounds__(PD_THREADS, WIDE ? (D == 128 ? 3 : 4) : (D == 128 ? 4 : 6)) PagedDecodeKernel(const TPagedDecodeParams p)
 {
-    constexpr int NT = D / 8;                       // column blocks of the output
+    constexpr int MT = D / 16;                      // row blocks of the output, 16 dimensions each
+    constexpr int HALVES = WIDE ? 2 : 1;            // blocks of eight query heads
     constexpr int KS = E4M3 ? D / 16 : D / 32;      // steps of the score product
     constexpr int ROWS = WIDE ? 16 : 8;
-    __shared__ float accOf[PD_WARPS][ROWS][D + 4]; // [.][.][4 (2 j + column) + t]: no two lanes of a store meet in a bank
+    __shared__ float accOf[PD_WARPS][ROWS][D + 4]; // [.][.][16 j + 2 g + b] for dimension D / 8 g + 2 j + b: no two lanes of a store meet in a bank
     __shared__ float refOf[PD_WARPS][ROWS], sumOf[PD_WARPS][ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const TPages &c = p.C;
@@ -275,10 +275,11 @@ __global__ void __launch_bounds__(PD_THREADS, D == 128 ? 3 : 5) PagedDecodeKerne
             }
         }
 
-        float acc[NT][4];
+        // acc[half][j]: heads 8 half + 2 t, + 1 (columns) of dimensions D / 8 g + 2 j (rows g), + 1 (rows g + 8)
+        float acc[HALVES][MT][4];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0;
+        for (int i = 0; i < HALVES * MT; ++i) {
+            acc[i / MT][i % MT][0] = acc[i / MT][i % MT][1] = acc[i / MT][i % MT][2] = acc[i / MT][i % MT][3] = 0;
         }
         float ref[2] = {PD_NO_REF, PD_NO_REF}, sum[2] = {0, 0};
 
@@ -394,13 +395,13 @@ __global__ void __launch_bounds__(PD_THREADS, D == 128 ? 3 : 5) PagedDecodeKerne
                     lv[i] = fmaxf(Log2(fabsf(vScale[i])), -100.0f);
                     const float bias = p.Slope * (float)(cur - place[i]);
 #pragma unroll
-                    for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+                    for (int half = 0; half < HALVES; ++half) {
                         z[half][i] = valid[i] ? z[half][i] * kScale[i] * mult[half] - bias : -INFINITY;
                     }
                 }
                 if (TRACK) {
 #pragma unroll
-                    for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+                    for (int half = 0; half < HALVES; ++half) {
                         if (g + 8 * half < rows) {
                             float *dst = p.Logits + ((size_t)seq * p.HeadCount + firstHead + g + 8 * half) * p.LogitRow + key0;
                             *reinterpret_cast<float4 *>(dst) = make_float4(z[half][0], z[half][1], z[half][2], z[half][3]);
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(PD_THREADS, D == 128 ? 3 : 5) PagedDecodeKerne
                 // raise the references of rows whose weights would leave f16's range
                 bool raise = false;
 #pragma unroll
-                for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+                for (int half = 0; half < HALVES; ++half) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         raise |= z[half][i] + lv[i] > ref[half] + 8.0f;
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(PD_THREADS, D == 128 ? 3 : 5) PagedDecodeKerne
                 if (__any_sync(0xffffffffu, raise)) {
                     float f[2] = {1, 1};
 #pragma unroll
-                    for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+                    for (int half = 0; half < HALVES; ++half) {
                         float m = ref[half];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -435,16 +436,20 @@ __global__ void __launch_bounds__(PD_THREADS, D == 128 ? 3 : 5) PagedDecodeKerne
                         sum[half] *= f[half];
                     }
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        acc[i][0] *= f[0];
-                        acc[i][1] *= f[0];
-                        acc[i][2] *= f[WIDE ? 1 : 0];
-                        acc[i][3] *= f[WIDE ? 1 : 0];
+                    for (int half = 0; half < HALVES; ++half) {
+                        const float f0 = __shfl_sync(0xffffffffu, f[half], 8 * t), f1 = __shfl_sync(0xffffffffu, f[half], 8 * t + 4);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            acc[half][i][0] *= f0;
+                            acc[half][i][1] *= f1;
+                            acc[half][i][2] *= f0;
+                            acc[half][i][3] *= f1;
+                        }
                     }
                 }
                 uint32_t hi[2][2], lo[2][2]; // [row half][keys 0, 1 / 2, 3]
 #pragma unroll
-                for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+                for (int half = 0; half < HALVES; ++half) {
                     float w[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -472,22 +477,25 @@ __global__ void __launch_bounds__(PD_THREADS, D == 128 ? 3 : 5) PagedDecodeKerne
                     const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), b01 = __byte_perm(x[0], x[1], 0x7362);
                     const uint32_t a23 = __byte_perm(x[2], x[3], 0x5140), b23 = __byte_perm(x[2], x[3], 0x7362);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t s01 = j < 2 ? a01 : b01, s23 = j < 2 ? a23 : b23;
-                        uint32_t b0, b1;
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t s01 = j ? b01 : a01, s23 = j ? b23 : a23;
+                        uint32_t a0, a1, a2, a3;
                         if (E4M3) {
-                            b0 = E4M3PairToF16(j & 1 ? s01 >> 16 : s01 & 0xffff);
-                            b1 = E4M3PairToF16(j & 1 ? s23 >> 16 : s23 & 0xffff);
+                            a0 = E4M3PairToF16(s01 & 0xffff);
+                            a1 = E4M3PairToF16(s01 >> 16);
+                            a2 = E4M3PairToF16(s23 & 0xffff);
+                            a3 = E4M3PairToF16(s23 >> 16);
                         } else {
-                            b0 = OffsetI8ToF16(s01, j & 1 ? 0x4342 : 0x4140);
-                            b1 = OffsetI8ToF16(s23, j & 1 ? 0x4342 : 0x4140);
+                            a0 = OffsetI8ToF16(s01, 0x4140);
+                            a1 = OffsetI8ToF16(s01, 0x4342);
+                            a2 = OffsetI8ToF16(s23, 0x4140);
+                            a3 = OffsetI8ToF16(s23, 0x4342);
                         }
-                        float(&o)[4] = acc[r * 4 + j];
-                        if (WIDE) {
-                            MmaF16(o, hi[0][0], hi[1][0], hi[0][1], hi[1][1], b0, b1);
-                            MmaF16(o, lo[0][0], lo[1][0], lo[0][1], lo[1][1], b0, b1);
-                        } else {
-                            MmaF16(o, hi[0][0], lo[0][0], hi[0][1], lo[0][1], b0, b1);
+#pragma unroll
+                        for (int half = 0; half < HALVES; ++half) {
+                            float(&o)[4] = acc[half][r * 2 + j];
+                            MmaF16(o, a0, a1, a2, a3, hi[half][0], hi[half][1]);
+                            MmaF16(o, a0, a1, a2, a3, lo[half][0], lo[half][1]);
                         }
                     }
                 }
@@ -499,28 +507,30 @@ __global__ void __launch_bounds__(PD_THREADS, D == 128 ? 3 : 5) PagedDecodeKerne
             }
         }
 
-        // the warps' sums meet in shared memory; lane (g, t) has dimensions D / 4 t .. of row g (column 2 t of every block, then column 2 t + 1)
+        // the warps' sums meet in shared memory
 #pragma unroll
-        for (int half = 0; half < (WIDE ? 2 : 1); ++half) {
+        for (int half = 0; half < HALVES; ++half) {
             sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 1);
             sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 2);
-            const int r = g + 8 * half;
             if (t == 0) {
-                refOf[warp][r] = ref[half];
-                sumOf[warp][r] = sum[half];
+                refOf[warp][g + 8 * half] = ref[half];
+                sumOf[warp][g + 8 * half] = sum[half];
             }
-            if (r < rows) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    accOf[warp][r][8 * j + t] = WIDE ? acc[j][2 * half] : acc[j][0] + acc[j][2];
-                    accOf[warp][r][8 * j + 4 + t] = WIDE ? acc[j][2 * half + 1] : acc[j][1] + acc[j][3];
+            for (int b = 0; b < 2; ++b) {
+                const int r = 8 * half + 2 * t + b;
+                if (r < rows) {
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) {
+                        *reinterpret_cast<float2 *>(&accOf[warp][r][16 * j + 2 * g]) = make_float2(acc[half][j][b], acc[half][j][2 + b]);
+                    }
                 }
             }
         }
         __syncthreads();
         for (int x = tid; x < rows * D; x += PD_THREADS) {
             const int r = x / D, i = x % D;
-            const int d = (i & 3) * (D / 4) + (i >> 2 & 1) * NT + (i >> 3);
+            const int d = (i >> 1 & 7) * (D / 8) + 2 * (i >> 4) + (i & 1);
             float m = refOf[0][r];
 #pragma unroll
             for (int w = 1; w < PD_WARPS; ++w) {
