@@ -27,6 +27,18 @@ __host__ __device__ __forceinline__ long long TableTokens(const TPages &c)
     return (long long)c.TableCols << c.PageShift;
 }
 
+__device__ __forceinline__ void ClusterSync()
+{
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// word of another CTA of the cluster at the place of `mine` in its shared memory
+__device__ __forceinline__ unsigned ClusterAddress(const void *mine, int rank)
+{
+    unsigned r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((unsigned)__cvta_generic_to_shared(mine)), "r"(rank));
+    return r;
+}
+
 // checks of the arguments that every entry point takes; needVectors: k, v and their scales have to be there
 int CheckPages(const char *fn, const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, int nSeq, bool needVectors, TPages *res);
 

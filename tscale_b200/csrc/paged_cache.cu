@@ -203,17 +203,6 @@ __device__ __forceinline__ uint4 SlotOrders(const TSelectParams &p, const int *t
     return o;
 }
 
-__device__ __forceinline__ void ClusterSync()
-{
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-// word of another CTA of the cluster at the place of `mine` in its shared memory
-__device__ __forceinline__ unsigned ClusterAddress(const void *mine, int rank)
-{
-    unsigned r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((unsigned)__cvta_generic_to_shared(mine)), "r"(rank));
-    return r;
-}
 __device__ __forceinline__ uint4 ClusterLoad16(unsigned address)
 {
     uint4 r;

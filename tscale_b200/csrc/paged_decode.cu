@@ -4,61 +4,34 @@
 //   out = sum_j 2^z_j * vScale_j * v_j / (1 + sum_j 2^z_j)                        (the 1: the sink of tsa_att_decode)
 //   weight_j += sum over the heads that share the key head of 2^z_j / (1 + sum)   (caches that keep weights)
 //
-// The stream of the cache bounds it: 2 D bytes of codes and two scales per key and key head, each read once.  The products run on the
-// warp's matrix instructions, scores = q K^T with the query heads of a key head as rows and result^T = V^T weights^T with them as columns,
-// so that up to 16 heads share what was loaded.  Fragments come straight from global memory: the order of the keys in a tile of 16 and of
-// the head's dimensions are free, and are taken such that every lane loads 16 bytes at a time (lane = 4 g + t), of
+// The stream of the cache bounds it: 2 D bytes of codes and two scales per key and key head, each read once; for short caches the latency
+// of what depends on one another does.  Two forms:
+//   clusters (here): a cluster of up to 8 CTAs has a unit (the up to 16 query heads that share a key head of a sequence) and joins its sums
+//     through distributed shared memory: one kernel, for caches of up to 4096 slots while all clusters are resident at once.
+//   ranges (paged_decode_sm100.cu): all keys of all units, in a row, are cut into equal ranges, one for each CTA that can be resident; a
+//     unit that a range border cuts leaves partial sums, which a second kernel joins in the order of the ranges.
+// No atomics in either: the same bits every time.
+//
+// Cluster form.  The products run on the warp's matrix instructions, scores = q K^T with the query heads as rows and result^T = V^T
+// weights^T with them as columns.  Fragments come straight from global memory: the order of the keys in a tile of 16 and of the head's
+// dimensions are free, and are taken such that every lane loads 16 bytes at a time (lane = 4 g + t), of
 //   K: key 4 (g / 2) + 2 n + g % 2 for column g of score block n, dimensions 16 t .. 16 t + 15 (and 64 more)
 //   V: keys 4 t .. 4 t + 3, dimensions D / 8 g .. D / 8 g + D / 8 - 1
 // which leaves lane (g, t) with the scores of head g for keys 4 t .. 4 t + 3: the weights are the second product's B fragment as they are.
-//
 // Weights: 2^(z - ref) * vScale in two f16 parts (22 bits; 2^-25 of the largest at worst), ref being the running maximum of
 // z + log2 |vScale|, raised when a tile exceeds it by 2^8.  int8 products are exact in int32; e4m3 codes are exact in f16 and their
 // products are summed in f32.
-//
-// Work: all keys of all (sequence, key head) units in a row, cut into equal ranges, one for each CTA that can be resident; a unit that a
-// range border cuts leaves partial sums, which a second kernel joins in the order of the ranges (no atomics: the same bits every time).
-#include "paged.cuh"
+#include "paged_decode.cuh"
+#include <type_traits>
 
 namespace tsa {
 
 constexpr int PD_WARPS = 4;
 constexpr int PD_THREADS = PD_WARPS * 32;
 constexpr int PD_TILE = 16;              // keys of a warp's tile
-constexpr int PD_MIN_TILES = 8;          // a CTA's range is at least two tiles per warp
-constexpr int PD_MAX_CTAS = 1024;
-constexpr int PD_ROWS = 16;              // query heads of a unit
-constexpr float PD_NO_REF = -1e30f;      // reference of sums that have no key yet
+constexpr int PD_MIN_TILES = 8;          // of a CTA: two tiles per warp
+constexpr int PD_MAX_CLUSTER = 8;
 
-struct TPagedDecodeParams {
-    TPages C;
-    const int *CtxLens, *Tokens;
-    int NSeq, HeadCount, Group, HeadChunks; // HeadChunks: units per key head (16 query heads each)
-    int Rows;                               // query heads of a unit's partial record
-    int MaxCtx, Window, OutDtype;
-    float Slope, DotScale, QVecScale;
-    P2D<uint8_t> Q;
-    P2D<float> QScale;
-    P2D<char> Out;
-    float *Partial;  // [CTA + unit][Rows][D + 4]: sums, reference, weight sum
-    float *Lse;      // [nSeq][heads]: log2 of the weights' sum and the sink (caches that keep weights)
-    float *Logits;   // [nSeq][heads][LogitRow]
-    int LogitRow;
-    int *Status;
-};
-
-__device__ __forceinline__ float Exp2(float x)
-{
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float Log2(float x)
-{
-    float r;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ uint4 LoadStream(const void *p)
 {
     uint4 r;
@@ -70,6 +43,14 @@ __device__ __forceinline__ uint2 LoadStream8(const void *p)
     uint2 r;
     asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
     return r;
+}
+__device__ __forceinline__ void LoadStream(const void *p, uint4 *r)
+{
+    *r = LoadStream(p);
+}
+__device__ __forceinline__ void LoadStream(const void *p, uint2 *r)
+{
+    *r = LoadStream8(p);
 }
 __device__ __forceinline__ void MmaS8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
@@ -109,72 +90,9 @@ __device__ __forceinline__ uint32_t PackRest(uint32_t hi, float a, float b)
     return PackHalf2(a - f.x, b - f.y);
 }
 
-// tiles [first, first + count) of 16 slots that hold the keys of a sequence; keys [beg, end) are slots when the cache has no positions
-struct TSeqKeys {
-    int First, Count, Beg, End;
-};
-__device__ __forceinline__ TSeqKeys SeqTiles(const TPagedDecodeParams &p, int s)
-{
-    const int len = p.CtxLens[s];
-    TSeqKeys r = {0, 0, 0, 0};
-    if (len <= 0 || len > p.MaxCtx || len > TableTokens(p.C)) {
-        return r;
-    }
-    r.End = len;
-    if (!p.C.Pos) {
-        const int cur = len - 1;
-        r.Beg = p.Window == 0 ? cur : max(0, cur - p.Window);
-        r.End = p.Window == 0 ? len : cur;
-    }
-    r.First = r.Beg / PD_TILE;
-    r.Count = r.End > r.Beg ? (r.End + PD_TILE - 1) / PD_TILE - r.First : 0;
-    return r;
-}
-
-// sum of the tiles of all sequences, by one warp; reports sequences that do not fit
-__device__ __forceinline__ int TotalTiles(const TPagedDecodeParams &p, int lane, bool report)
-{
-    int sum = 0;
-    for (int s = lane; s < p.NSeq; s += 32) {
-        sum += SeqTiles(p, s).Count;
-        if (report && p.Status && (p.CtxLens[s] > p.MaxCtx || p.CtxLens[s] > TableTokens(p.C))) {
-            atomicOr(p.Status, kDevBadSpan);
-        }
-    }
-    return __reduce_add_sync(0xffffffffu, sum);
-}
-
-// the sequence that holds tile `at` of the row of all sequences' tiles, each `mult` times; *base: the tile where it begins
-__device__ __forceinline__ int SeqOfTile(const TPagedDecodeParams &p, unsigned at, int mult, int lane, unsigned *base)
-{
-    unsigned before = 0;
-    for (int s0 = 0; s0 < p.NSeq; s0 += 32) {
-        const unsigned mine = s0 + lane < p.NSeq ? SeqTiles(p, s0 + lane).Count * mult : 0;
-        unsigned sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned v = __shfl_up_sync(0xffffffffu, sum, o);
-            sum += lane >= o ? v : 0;
-        }
-        const unsigned in = __ballot_sync(0xffffffffu, before + sum > at);
-        if (in) {
-            const int l = __ffs(in) - 1;
-            *base = before + __shfl_sync(0xffffffffu, sum - mine, l);
-            return s0 + l;
-        }
-        before += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    return -1;
-}
-
-// tiles of a CTA's range
-__device__ __forceinline__ unsigned RangeTiles(unsigned total, unsigned ctas)
-{
-    return max((total + ctas - 1) / ctas, (unsigned)PD_MIN_TILES);
-}
-
+// scales of four keys
 template <bool F16>
-struct TScales; // scales of four keys
+struct TScales;
 template <>
 struct TScales<true> {
     uint2 X;
@@ -192,270 +110,303 @@ struct TScales<false> {
     __device__ __forceinline__ float Get(int i) const { return __uint_as_float(i == 0 ? X.x : i == 1 ? X.y : i == 2 ? X.z : X.w); }
 };
 
-// WIDE: more than eight query heads share a key head (otherwise rows 8 .. 15 of the scores are unused, and half the sums).
-// SINGLE: a CTA has one whole unit (short contexts): no ranges, no partial sums, no second kernel.
-template <int D, bool E4M3, bool SCALE_F16, bool WIDE, bool TRACK, bool SINGLE>
-__global__ void __launch_bounds__(PD_THREADS, WIDE ? (D == 128 ? 3 : 4) : (D == 128 ? 4 : 6)) PagedDecodeKernel(const TPagedDecodeParams p)
+__device__ __forceinline__ float ClusterLoad(const float *mine, int rank)
 {
+    float r;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r) : "r"(ClusterAddress(mine, rank)) : "memory");
+    return r;
+}
+
+// One cluster of p.Cluster CTAs per unit.  WIDE: more than eight query heads share a key head (otherwise rows 8 .. 15 of the scores are
+// unused, and half the sums).  A warp works on U tiles of 16 keys at a time, 4 KB of K and V, and holds the loads of its next ones in
+// registers meanwhile.
+template <int D, bool E4M3, bool SCALE_F16, bool WIDE>
+__global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(const TPagedDecodeParams p)
+{
+    constexpr int U = 128 / D, STEP = PD_WARPS * U;
     constexpr int MT = D / 16;                      // row blocks of the output, 16 dimensions each
     constexpr int HALVES = WIDE ? 2 : 1;            // blocks of eight query heads
     constexpr int KS = E4M3 ? D / 16 : D / 32;      // steps of the score product
-    constexpr int ROWS = WIDE ? 16 : 8;
-    __shared__ float accOf[PD_WARPS][ROWS][D + 4]; // [.][.][16 j + 2 g + b] for dimension D / 8 g + 2 j + b: no two lanes of a store meet in a bank
-    __shared__ float refOf[PD_WARPS][ROWS], sumOf[PD_WARPS][ROWS];
+    constexpr int ROWS = 8 * HALVES;
+    typedef typename std::conditional<D == 128, uint4, uint2>::type TPiece; // D / 8 dimensions of a key
+    __shared__ __align__(16) float accOf[PD_WARPS][ROWS][D + 4]; // [.][.][16 j + 2 g + b] for dimension D / 8 g + 2 j + b: no two lanes of a store meet in a bank
+    __shared__ float refOf[PD_WARPS][ROWS], sumOf[PD_WARPS][ROWS], lseOf[ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const TPages &c = p.C;
-    const int unitsPerSeq = c.KvHeads * p.HeadChunks;
+    const int unitsPerSeq = c.KvHeads * p.HeadChunks, ctas = p.Cluster, rank = blockIdx.x % ctas, unit = blockIdx.x / ctas;
+    const int seq = unit / unitsPerSeq, head = unit % unitsPerSeq / p.HeadChunks, chunk = unit % p.HeadChunks;
+    const int firstHead = head * p.Group + chunk * PD_ROWS, rows = min(p.Group - chunk * PD_ROWS, PD_ROWS);
     PdlWait();
     PdlTrigger();
-
-    unsigned at, rangeEnd, per = 0;
-    int seq;
-    unsigned seqBase;
-    if (SINGLE) {
-        seq = blockIdx.x / unitsPerSeq;
-        const int n = SeqTiles(p, seq).Count;
-        seqBase = 0;
-        at = (blockIdx.x % unitsPerSeq) * n;
-        rangeEnd = at + n;
-        if (tid == 0 && p.Status && (p.CtxLens[seq] > p.MaxCtx || p.CtxLens[seq] > TableTokens(c))) {
-            atomicOr(p.Status, kDevBadSpan);
-        }
-    } else {
-        const unsigned total = (unsigned)TotalTiles(p, lane, blockIdx.x == 0 && warp == 0) * unitsPerSeq;
-        per = RangeTiles(total, gridDim.x);
-        at = blockIdx.x * per;
-        rangeEnd = min(at + per, total);
-        if (at >= rangeEnd) {
-            return;
-        }
-        seq = SeqOfTile(p, at, unitsPerSeq, lane, &seqBase);
+    if (tid == 0 && p.Status && (p.CtxLens[seq] > p.MaxCtx || p.CtxLens[seq] > TableTokens(c))) {
+        atomicOr(p.Status, kDevBadSpan);
     }
-    bool badPage = false;
-    // one turn per unit that the range touches
-    do {
-        const TSeqKeys keys = SeqTiles(p, seq);
-        const int inSeq = SINGLE ? (int)(blockIdx.x % unitsPerSeq) : (int)((at - seqBase) / keys.Count);
-        const int head = inSeq / p.HeadChunks, chunk = inSeq % p.HeadChunks;
-        const unsigned unitBeg = seqBase + (unsigned)inSeq * keys.Count;
-        const int segBeg = keys.First + (int)(at - unitBeg), segEnd = keys.First + (int)(min(rangeEnd, unitBeg + keys.Count) - unitBeg);
-        const bool whole = segBeg == keys.First && segEnd == keys.First + keys.Count;
-        const int firstHead = head * p.Group + chunk * PD_ROWS;
-        const int rows = min(p.Group - chunk * PD_ROWS, PD_ROWS);
-        const int cur = (p.Tokens ? p.Tokens[seq] : p.CtxLens[seq]) - 1;
-        const int *table = c.Table.Row(seq);
-        const int tileShift = c.PageShift - 4, tileMask = (1 << tileShift) - 1;
+    const TSeqKeys keys = SeqTiles<PD_TILE>(p, seq);
+    const int per = (keys.Count + ctas - 1) / ctas;
+    const int segBeg = keys.First + min(rank * per, keys.Count), segEnd = min(segBeg + per, keys.First + keys.Count);
+    const int cur = (p.Tokens ? p.Tokens[seq] : p.CtxLens[seq]) - 1;
+    const int *table = c.Table.Row(seq);
+    const int tileShift = c.PageShift - 4, tileMask = (1 << tileShift) - 1;
+    // keys of this CTA; a key at distance cur - position is attended if (unsigned)(distance - nearest) < spread
+    const int keyBeg = keys.Beg, keyEnd = min(keys.End, segEnd * PD_TILE);
+    const int nearest = p.Window > 0 ? 1 : 0;
+    const unsigned spread = p.Window > 0 ? p.Window : 1;
+    float *const logits = p.Logits ? p.Logits + ((size_t)seq * p.HeadCount + firstHead) * p.LogitRow : nullptr;
 
-        // the query heads of this lane's rows, in the dimensions' order of the fragments
-        uint32_t qa[KS][4];
-        float mult[2] = {0, 0};
+    // the query heads of this lane's rows, in the dimensions' order of the fragments
+    uint32_t qa[KS][4];
+    float mult[2] = {0, 0};
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int r = g + 8 * half;
-            const bool live = (half == 0 || WIDE) && r < rows;
-            uint32_t w[D / 16];
+    for (int half = 0; half < 2; ++half) {
+        const int r = g + 8 * half;
+        const bool live = half < HALVES && r < rows;
+        uint32_t w[D / 16];
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (live) {
-                    x = *reinterpret_cast<const uint4 *>(p.Q.Row(seq) + (firstHead + r) * D + i * 64 + t * 16);
-                }
-                w[i * 4 + 0] = x.x;
-                w[i * 4 + 1] = x.y;
-                w[i * 4 + 2] = x.z;
-                w[i * 4 + 3] = x.w;
-            }
+        for (int i = 0; i < D / 64; ++i) {
+            uint4 x = make_uint4(0, 0, 0, 0);
             if (live) {
-                mult[half] = p.DotScale * (p.QScale.Valid() ? p.QScale.Row(seq)[firstHead + r] : p.QVecScale);
+                x = *reinterpret_cast<const uint4 *>(p.Q.Row(seq) + (firstHead + r) * D + i * 64 + t * 16);
             }
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                qa[i][half] = E4M3 ? E4M3PairToF16(w[E4M3 ? i : 0] & 0xffff) : w[E4M3 ? 0 : 2 * i];
-                qa[i][half + 2] = E4M3 ? E4M3PairToF16(w[E4M3 ? i : 0] >> 16) : w[E4M3 ? 0 : 2 * i + 1];
-            }
+            w[i * 4 + 0] = x.x;
+            w[i * 4 + 1] = x.y;
+            w[i * 4 + 2] = x.z;
+            w[i * 4 + 3] = x.w;
         }
-
-        // acc[half][j]: heads 8 half + 2 t, + 1 (columns) of dimensions D / 8 g + 2 j (rows g), + 1 (rows g + 8)
-        float acc[HALVES][MT][4];
-#pragma unroll
-        for (int i = 0; i < HALVES * MT; ++i) {
-            acc[i / MT][i % MT][0] = acc[i / MT][i % MT][1] = acc[i / MT][i % MT][2] = acc[i / MT][i % MT][3] = 0;
+        if (live) {
+            mult[half] = p.DotScale * (p.QScale.Valid() ? p.QScale.Row(seq)[firstHead + r] : p.QVecScale);
         }
-        float ref[2] = {PD_NO_REF, PD_NO_REF}, sum[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            qa[i][half] = E4M3 ? E4M3PairToF16(w[E4M3 ? i : 0] & 0xffff) : w[E4M3 ? 0 : 2 * i];
+            qa[i][half + 2] = E4M3 ? E4M3PairToF16(w[E4M3 ? i : 0] >> 16) : w[E4M3 ? 0 : 2 * i + 1];
+        }
+    }
 
-        uint4 kr[2][D / 64];
-        uint4 vr[4]; // D = 64 uses the first halves
-        TScales<SCALE_F16> ks, vs;
-        int4 ps;
-        bool pageOk = true;
-        const int keyRow = 4 * (g >> 1) + (g & 1); // of score block 0
-        auto pageOf = [&](int tile) { return tile < segEnd ? table[tile >> tileShift] : 0; };
-        auto slotOf = [&](int tile, int page) {
-            pageOk = (unsigned)page < (unsigned)c.PageCount;
-            return PlaneSlot(c, pageOk ? page : 0, head) + ((tile & tileMask) << 4);
-        };
-        auto loadK = [&](size_t slot) {
+    // acc[half][j]: heads 8 half + 2 t, + 1 (columns) of dimensions D / 8 g + 2 j (rows g), + 1 (rows g + 8)
+    float acc[HALVES][MT][4];
+#pragma unroll
+    for (int i = 0; i < HALVES * MT; ++i) {
+        acc[i / MT][i % MT][0] = acc[i / MT][i % MT][1] = acc[i / MT][i % MT][2] = acc[i / MT][i % MT][3] = 0;
+    }
+    float ref[HALVES], sum[HALVES];
+#pragma unroll
+    for (int half = 0; half < HALVES; ++half) {
+        ref[half] = PD_NO_REF;
+        sum[half] = 0;
+    }
+
+    uint4 kr[U][2][D / 64];
+    TPiece vr[U][4];
+    TScales<SCALE_F16> ks[U], vs[U];
+    int4 ps[U];
+    const int keyRow = 4 * (g >> 1) + (g & 1); // of score block 0
+    const size_t kLane = (size_t)keyRow * D + t * 16, vLane = (size_t)(4 * t) * D + g * (D / 8);
+    auto pageOf = [&](int tile) { return tile < segEnd ? table[tile >> tileShift] : -1; };
+    // the slots of a tile; a tile that there is not, or whose page is outside the pool, reads page 0 and is masked
+    auto slotOf = [&](int tile, int page) {
+        return PlaneSlot(c, (unsigned)page < (unsigned)c.PageCount ? page : 0, head) + ((tile & tileMask) << 4);
+    };
+    auto loadK = [&](const size_t (&slot)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint8_t *src = c.K + slot[u] * D + kLane;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
 #pragma unroll
                 for (int i = 0; i < D / 64; ++i) {
-                    kr[n][i] = LoadStream(c.K + (slot + keyRow + 2 * n) * D + i * 64 + t * 16);
+                    kr[u][n][i] = LoadStream(src + 2 * n * D + i * 64);
                 }
             }
-            ks.Load(c.KScale, slot + 4 * t);
+            ks[u].Load(c.KScale, slot[u] + 4 * t);
+            vs[u].Load(c.VScale, slot[u] + 4 * t); // with K: the weights need it before V
             if (c.Pos) {
-                ps = *reinterpret_cast<const int4 *>(c.Pos + slot + 4 * t);
+                ps[u] = *reinterpret_cast<const int4 *>(c.Pos + slot[u] + 4 * t);
             }
-        };
-        auto loadV = [&](size_t slot) {
+        }
+    };
+    auto loadV = [&](const size_t (&slot)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint8_t *src = c.V + slot[u] * D + vLane;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint8_t *src = c.V + (slot + 4 * t + i) * D + g * (D / 8);
-                if (D == 128) {
-                    vr[i] = LoadStream(src);
-                } else {
-                    const uint2 x = LoadStream8(src);
-                    vr[i].x = x.x;
-                    vr[i].y = x.y;
-                }
+                LoadStream(src + i * D, &vr[u][i]);
             }
-            vs.Load(c.VScale, slot + 4 * t);
-        };
+        }
+    };
 
-        int tile = segBeg + warp;
-        if (tile < segEnd) {
-            size_t slot = slotOf(tile, pageOf(tile));
-            bool okNow = pageOk;
-            loadK(slot);
-            loadV(slot);
-            int pageNext = pageOf(tile + PD_WARPS);
-            for (; tile < segEnd; tile += PD_WARPS) {
-                const bool more = tile + PD_WARPS < segEnd;
-                const size_t slotNext = more ? slotOf(tile + PD_WARPS, pageNext) : slot;
-                const bool okNext = pageOk;
-                pageNext = pageOf(tile + 2 * PD_WARPS);
-                badPage |= !okNow;
+    bool badPage = false;
+    int tile = segBeg + warp * U;
+    if (tile < segEnd) {
+        size_t slot[U];
+        int page[U];
+        bool ok[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            page[u] = pageOf(tile + u);
+            slot[u] = slotOf(tile + u, page[u]);
+            ok[u] = (unsigned)page[u] < (unsigned)c.PageCount;
+            badPage |= !ok[u] && tile + u < segEnd;
+        }
+        loadK(slot);
+        loadV(slot);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            page[u] = pageOf(tile + STEP + u);
+        }
+        for (; tile < segEnd; tile += STEP) {
+            const bool more = tile + STEP < segEnd;
+            bool okNow[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                okNow[u] = ok[u];
+                if (more) {
+                    slot[u] = slotOf(tile + STEP + u, page[u]);
+                    ok[u] = (unsigned)page[u] < (unsigned)c.PageCount;
+                    badPage |= !ok[u] && tile + STEP + u < segEnd;
+                }
+                page[u] = pageOf(tile + 2 * STEP + u);
+            }
 
-                // scores of block n, columns 2 t and 2 t + 1: keys 4 t + 2 n and 4 t + 2 n + 1
-                float z[2][4]; // [row half][key]
+            // scores of block n, columns 2 t and 2 t + 1: keys 4 t + 2 n and 4 t + 2 n + 1; then logits
+            float z[U][HALVES][4], vScale[U][4], edge[U][4];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
+                    float dot[4];
                     if (E4M3) {
                         float d[4] = {0, 0, 0, 0};
 #pragma unroll
-                        for (int i = 0; i < D / 64; ++i) {
-                            const uint32_t w[4] = {kr[n][i].x, kr[n][i].y, kr[n][i].z, kr[n][i].w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint32_t(&a)[4] = qa[E4M3 ? i * 4 + j : 0];
-                                MmaF16(d, a[0], a[1], a[2], a[3], E4M3PairToF16(w[j] & 0xffff), E4M3PairToF16(w[j] >> 16));
-                            }
+                        for (int i = 0; i < KS; ++i) {
+                            const uint32_t w = reinterpret_cast<const uint32_t *>(&kr[u][n][E4M3 ? i / 4 : 0])[i % 4];
+                            MmaF16(d, qa[i][0], qa[i][1], qa[i][2], qa[i][3], E4M3PairToF16(w & 0xffff), E4M3PairToF16(w >> 16));
                         }
-                        z[0][2 * n] = d[0];
-                        z[0][2 * n + 1] = d[1];
-                        z[1][2 * n] = d[2];
-                        z[1][2 * n + 1] = d[3];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            dot[i] = d[i];
+                        }
                     } else {
                         int d[4] = {0, 0, 0, 0};
 #pragma unroll
-                        for (int i = 0; i < D / 64; ++i) {
-                            MmaS8(d, qa[E4M3 ? 0 : 2 * i], kr[n][i].x, kr[n][i].y);
-                            MmaS8(d, qa[E4M3 ? 0 : 2 * i + 1], kr[n][i].z, kr[n][i].w);
+                        for (int i = 0; i < KS; ++i) {
+                            const uint4 &k4 = kr[u][n][E4M3 ? 0 : i / 2];
+                            MmaS8(d, qa[i], i % 2 ? k4.z : k4.x, i % 2 ? k4.w : k4.y);
                         }
-                        z[0][2 * n] = (float)d[0];
-                        z[0][2 * n + 1] = (float)d[1];
-                        z[1][2 * n] = (float)d[2];
-                        z[1][2 * n + 1] = (float)d[3];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            dot[i] = (float)d[i];
+                        }
+                    }
+#pragma unroll
+                    for (int half = 0; half < HALVES; ++half) {
+                        z[u][half][2 * n] = dot[2 * half];
+                        z[u][half][2 * n + 1] = dot[2 * half + 1];
                     }
                 }
-                float kScale[4], vScale[4], lv[4];
-                const int key0 = tile * PD_TILE + 4 * t;
-                const int place[4] = {c.Pos ? ps.x : key0, c.Pos ? ps.y : key0 + 1, c.Pos ? ps.z : key0 + 2, c.Pos ? ps.w : key0 + 3};
-                // a tile in the middle of the range of a cache without positions has no masked key
-                const bool plain = okNow && !c.Pos && tile * PD_TILE >= keys.Beg && (tile + 1) * PD_TILE <= keys.End;
-                bool valid[4] = {true, true, true, true};
-                if (!plain) {
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int key0 = (tile + u) * PD_TILE + 4 * t;
+                int far[4] = {cur - key0, cur - key0 - 1, cur - key0 - 2, cur - key0 - 3};
+                if (c.Pos) {
+                    far[0] = cur - ps[u].x;
+                    far[1] = cur - ps[u].y;
+                    far[2] = cur - ps[u].z;
+                    far[3] = cur - ps[u].w;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    vScale[u][i] = vs[u].Get(i);
+                    const float kScale = ks[u].Get(i);
+#pragma unroll
+                    for (int half = 0; half < HALVES; ++half) {
+                        z[u][half][i] *= kScale * mult[half];
+                    }
+                }
+                if (p.Slope != 0) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int key = key0 + i;
-                        valid[i] = okNow && key >= keys.Beg && key < keys.End;
-                        if (c.Pos) {
-                            const int far = cur - place[i];
-                            valid[i] = valid[i] && (p.Window == 0 ? far == 0 : far >= 1 && far <= p.Window);
+#pragma unroll
+                        for (int half = 0; half < HALVES; ++half) {
+                            z[u][half][i] = fmaf(-p.Slope, (float)far[i], z[u][half][i]);
                         }
-                        if (E4M3 && !valid[i]) {
-                            vr[i] = make_uint4(0, 0, 0, 0); // what is in the slot may be NaN
+                    }
+                }
+                // a tile in the middle of the range of a cache without positions has no masked key
+                if (!okNow[u] || c.Pos || (tile + u) * PD_TILE < keyBeg || (tile + u + 1) * PD_TILE > keyEnd) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool valid = okNow[u] && key0 + i >= keyBeg && key0 + i < keyEnd && (unsigned)(far[i] - nearest) < spread;
+                        if (!valid) { // what is in the slot may be NaN
+                            vScale[u][i] = 0;
+                            if (E4M3) {
+                                vr[u][i] = TPiece{};
+                            }
+#pragma unroll
+                            for (int half = 0; half < HALVES; ++half) {
+                                z[u][half][i] = -INFINITY;
+                            }
+                        }
+                    }
+                }
+                if (logits && tile + u < segEnd) {
+#pragma unroll
+                    for (int half = 0; half < HALVES; ++half) {
+                        if (g + 8 * half < rows) {
+                            *reinterpret_cast<float4 *>(logits + (size_t)(g + 8 * half) * p.LogitRow + key0) =
+                                make_float4(z[u][half][0], z[u][half][1], z[u][half][2], z[u][half][3]);
                         }
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    kScale[i] = ks.Get(i);
-                    vScale[i] = valid[i] ? vs.Get(i) : 0.0f;
-                    lv[i] = fmaxf(Log2(fabsf(vScale[i])), -100.0f);
-                    const float bias = p.Slope * (float)(cur - place[i]);
+                    edge[u][i] = ReferenceEdge(vScale[u][i]);
+                }
+            }
+            if (more) {
+                loadK(slot);
+            }
+            // raise the references of rows whose weights would leave f16's range
+            bool raise = false;
 #pragma unroll
-                    for (int half = 0; half < HALVES; ++half) {
-                        z[half][i] = valid[i] ? z[half][i] * kScale[i] * mult[half] - bias : -INFINITY;
-                    }
-                }
-                if (TRACK) {
-#pragma unroll
-                    for (int half = 0; half < HALVES; ++half) {
-                        if (g + 8 * half < rows) {
-                            float *dst = p.Logits + ((size_t)seq * p.HeadCount + firstHead + g + 8 * half) * p.LogitRow + key0;
-                            *reinterpret_cast<float4 *>(dst) = make_float4(z[half][0], z[half][1], z[half][2], z[half][3]);
-                        }
-                    }
-                }
-                if (more) {
-                    loadK(slotNext);
-                }
-                // raise the references of rows whose weights would leave f16's range
-                bool raise = false;
+            for (int i = 0; i < U * HALVES * 4; ++i) {
+                raise |= z[i / 4 / HALVES][i / 4 % HALVES][i % 4] - ref[i / 4 % HALVES] > edge[i / 4 / HALVES][i % 4];
+            }
+            if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int half = 0; half < HALVES; ++half) {
+                    float m = ref[half];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        raise |= z[half][i] + lv[i] > ref[half] + 8.0f;
+                    for (int i = 0; i < U * 4; ++i) {
+                        m = fmaxf(m, z[i / 4][half][i % 4] - edge[i / 4][i % 4] + 8.0f);
+                    }
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    const float f = Exp2(ref[half] - m);
+                    ref[half] = m;
+                    sum[half] *= f;
+                    const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        acc[half][i][0] *= f0;
+                        acc[half][i][1] *= f1;
+                        acc[half][i][2] *= f0;
+                        acc[half][i][3] *= f1;
                     }
                 }
-                if (__any_sync(0xffffffffu, raise)) {
-                    float f[2] = {1, 1};
+            }
 #pragma unroll
-                    for (int half = 0; half < HALVES; ++half) {
-                        float m = ref[half];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            m = fmaxf(m, z[half][i] + lv[i]);
-                        }
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                        f[half] = Exp2(ref[half] - m);
-                        ref[half] = m;
-                        sum[half] *= f[half];
-                    }
-#pragma unroll
-                    for (int half = 0; half < HALVES; ++half) {
-                        const float f0 = __shfl_sync(0xffffffffu, f[half], 8 * t), f1 = __shfl_sync(0xffffffffu, f[half], 8 * t + 4);
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            acc[half][i][0] *= f0;
-                            acc[half][i][1] *= f1;
-                            acc[half][i][2] *= f0;
-                            acc[half][i][3] *= f1;
-                        }
-                    }
-                }
-                uint32_t hi[2][2], lo[2][2]; // [row half][keys 0, 1 / 2, 3]
+            for (int u = 0; u < U; ++u) {
+                uint32_t hi[HALVES][2], lo[HALVES][2]; // [.][keys 0, 1 / 2, 3]
 #pragma unroll
                 for (int half = 0; half < HALVES; ++half) {
                     float w[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        w[i] = Exp2(z[half][i] - ref[half]);
+                        w[i] = Exp2(z[u][half][i] - ref[half]);
                         sum[half] += w[i];
-                        w[i] *= vScale[i];
+                        w[i] *= vScale[u][i];
                     }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -469,16 +420,14 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? (D == 128 ? 3 : 4) : (D == 
                     uint32_t x[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[i] = r == 0 ? vr[i].x : r == 1 ? vr[i].y : r == 2 ? vr[i].z : vr[i].w;
+                        x[i] = reinterpret_cast<const uint32_t *>(&vr[u][i])[r];
                         if (!E4M3) {
                             x[i] ^= 0x80808080u;
                         }
                     }
-                    const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), b01 = __byte_perm(x[0], x[1], 0x7362);
-                    const uint32_t a23 = __byte_perm(x[2], x[3], 0x5140), b23 = __byte_perm(x[2], x[3], 0x7362);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const uint32_t s01 = j ? b01 : a01, s23 = j ? b23 : a23;
+                        const uint32_t s01 = __byte_perm(x[0], x[1], j ? 0x7362 : 0x5140), s23 = __byte_perm(x[2], x[3], j ? 0x7362 : 0x5140);
                         uint32_t a0, a1, a2, a3;
                         if (E4M3) {
                             a0 = E4M3PairToF16(s01 & 0xffff);
@@ -499,83 +448,92 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? (D == 128 ? 3 : 4) : (D == 
                         }
                     }
                 }
-                if (more) {
-                    loadV(slotNext);
-                }
-                slot = slotNext;
-                okNow = okNext;
+            }
+            if (more) {
+                loadV(slot);
             }
         }
-
-        // the warps' sums meet in shared memory
-#pragma unroll
-        for (int half = 0; half < HALVES; ++half) {
-            sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 1);
-            sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 2);
-            if (t == 0) {
-                refOf[warp][g + 8 * half] = ref[half];
-                sumOf[warp][g + 8 * half] = sum[half];
-            }
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int r = 8 * half + 2 * t + b;
-                if (r < rows) {
-#pragma unroll
-                    for (int j = 0; j < MT; ++j) {
-                        *reinterpret_cast<float2 *>(&accOf[warp][r][16 * j + 2 * g]) = make_float2(acc[half][j][b], acc[half][j][2 + b]);
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        for (int x = tid; x < rows * D; x += PD_THREADS) {
-            const int r = x / D, i = x % D;
-            const int d = (i >> 1 & 7) * (D / 8) + 2 * (i >> 4) + (i & 1);
-            float m = refOf[0][r];
-#pragma unroll
-            for (int w = 1; w < PD_WARPS; ++w) {
-                m = fmaxf(m, refOf[w][r]);
-            }
-            float s = 0, a = 0;
-#pragma unroll
-            for (int w = 0; w < PD_WARPS; ++w) {
-                const float f = Exp2(refOf[w][r] - m);
-                s = fmaf(f, sumOf[w][r], s);
-                a = fmaf(f, accOf[w][r][i], a);
-            }
-            if (whole) {
-                // the sink: weight 1 at logit 0
-                const float all = fmaxf(m, -60.0f), f = Exp2(m - all);
-                s = fmaf(f, s, Exp2(-all));
-                StoreFromFloat(p.Out.Row(seq), (firstHead + r) * D + d, p.OutDtype, a * f / s);
-                if (TRACK && d == 0) {
-                    p.Lse[(size_t)seq * p.HeadCount + firstHead + r] = all + Log2(s);
-                }
-            } else {
-                float *dst = p.Partial + ((size_t)(blockIdx.x + seq * unitsPerSeq + inSeq) * p.Rows + r) * (D + 4);
-                dst[d] = a;
-                if (d == 0) {
-                    dst[D] = m;
-                    dst[D + 1] = s;
-                }
-            }
-        }
-        if (SINGLE) {
-            break;
-        }
-        at = unitBeg + (segEnd - keys.First);
-        if (at < rangeEnd) {
-            __syncthreads(); // shared memory is free again
-            if (at == seqBase + (unsigned)keys.Count * unitsPerSeq) {
-                seqBase = at;
-                do {
-                    ++seq;
-                } while (SeqTiles(p, seq).Count == 0);
-            }
-        }
-    } while (at < rangeEnd);
+    }
     if (badPage && p.Status) {
         atomicOr(p.Status, kDevBadSpan);
+    }
+
+    // the warps' sums meet in shared memory
+#pragma unroll
+    for (int half = 0; half < HALVES; ++half) {
+        sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 1);
+        sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 2);
+        if (t == 0) {
+            refOf[warp][g + 8 * half] = ref[half];
+            sumOf[warp][g + 8 * half] = sum[half];
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int r = 8 * half + 2 * t + b;
+            if (r < rows) {
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    *reinterpret_cast<float2 *>(&accOf[warp][r][16 * j + 2 * g]) = make_float2(acc[half][j][b], acc[half][j][2 + b]);
+                }
+            }
+        }
+    }
+    if (ctas > 1) {
+        // each CTA of the cluster finishes a part of the result from all their sums
+        ClusterSync();
+    } else {
+        __syncthreads();
+    }
+    auto refAt = [&](int i, int r) { return ctas > 1 ? ClusterLoad(&refOf[i % PD_WARPS][r], i / PD_WARPS) : refOf[i][r]; };
+    auto sumAt = [&](int i, int r) { return ctas > 1 ? ClusterLoad(&sumOf[i % PD_WARPS][r], i / PD_WARPS) : sumOf[i][r]; };
+    auto accAt = [&](int i, int r, int x) { return ctas > 1 ? ClusterLoad(&accOf[i % PD_WARPS][r][x], i / PD_WARPS) : accOf[i][r][x]; };
+    // reference of all warps' sums of row r (at least -60: then the sink, weight 1 at logit 0, stays in range) and their weights' sum
+    auto joined = [&](int r, float *sumAll) {
+        float m = -60.0f;
+#pragma unroll 4
+        for (int w = 0; w < PD_WARPS * ctas; ++w) {
+            m = fmaxf(m, refAt(w, r));
+        }
+        float s = Exp2(-m);
+#pragma unroll 4
+        for (int w = 0; w < PD_WARPS * ctas; ++w) {
+            s = fmaf(Exp2(refAt(w, r) - m), sumAt(w, r), s);
+        }
+        *sumAll = s;
+        return m;
+    };
+    for (int x = rank * PD_THREADS + tid; x < rows * D; x += ctas * PD_THREADS) {
+        const int r = x / D, i = x % D;
+        const int d = (i >> 1 & 7) * (D / 8) + 2 * (i >> 4) + (i & 1);
+        float s, a = 0;
+        const float m = joined(r, &s);
+#pragma unroll 4
+        for (int w = 0; w < PD_WARPS * ctas; ++w) {
+            a = fmaf(Exp2(refAt(w, r) - m), accAt(w, r, i), a);
+        }
+        StoreFromFloat(p.Out.Row(seq), (firstHead + r) * D + d, p.OutDtype, a / s);
+    }
+    if (logits) {
+        // the weights of this CTA's keys (one unit per key head: nobody else adds to them)
+        if (tid < rows) {
+            float s;
+            const float m = joined(tid, &s);
+            lseOf[tid] = m + Log2(s);
+        }
+        __syncthreads();
+        for (int key = max(keyBeg, segBeg * PD_TILE) + tid; key < keyEnd; key += PD_THREADS) {
+            const int page = table[key >> c.PageShift];
+            if ((unsigned)page < (unsigned)c.PageCount) {
+                float w = 0;
+                for (int r = 0; r < rows; ++r) {
+                    w += Exp2(logits[(size_t)r * p.LogitRow + key] - lseOf[r]);
+                }
+                c.Weight[PlaneSlot(c, page, head) + (key & ((1 << c.PageShift) - 1))] += w;
+            }
+        }
+    }
+    if (ctas > 1) {
+        ClusterSync(); // no CTA leaves while another reads its shared memory
     }
 }
 
@@ -584,7 +542,7 @@ __device__ __forceinline__ void SeqStart(const TPagedDecodeParams &p, int seq, i
 {
     int before = 0, all = 0;
     for (int s = lane; s < p.NSeq; s += 32) {
-        const int n = SeqTiles(p, s).Count;
+        const int n = SeqTiles<PD_RANGE_TILE>(p, s).Count;
         before += s < seq ? n : 0;
         all += n;
     }
@@ -604,11 +562,11 @@ __global__ void __launch_bounds__(128) PagedJoinKernel(const TPagedDecodeParams 
     __shared__ float4 sumAcc[GROUPS][LPC];
     const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
     const int kvHead = head / p.Group, inGroup = head % p.Group, chunk = inGroup / PD_ROWS, row = inGroup % PD_ROWS;
-    const int units = p.C.KvHeads * p.HeadChunks, inSeq = kvHead * p.HeadChunks + chunk;
+    const int inSeq = kvHead * p.HeadChunks + chunk;
     unsigned start, per;
     // the lengths were there before the kernel whose sums are joined began
     SeqStart(p, seq, lane, ctas, &start, &per);
-    const int count = SeqTiles(p, seq).Count;
+    const int count = SeqTiles<PD_RANGE_TILE>(p, seq).Count;
     PdlWait();
     PdlTrigger();
     if (count == 0) {
@@ -627,7 +585,7 @@ __global__ void __launch_bounds__(128) PagedJoinKernel(const TPagedDecodeParams 
     }
     const int chunks = c1 - c0 + 1;
     const size_t stride = (size_t)p.Rows * (D + 4);
-    const float *base = p.Partial + (size_t)(c0 + seq * units + inSeq) * stride + (size_t)row * (D + 4);
+    const float *base = PartialRecord(p, D, c0, seq, inSeq, row);
     float m = -60.0f;
     for (int i = tid; i < chunks; i += 128) {
         m = fmaxf(m, base[i * stride + D]);
@@ -680,8 +638,8 @@ __global__ void __launch_bounds__(256) PagedWeightKernel(const TPagedDecodeParam
     PdlWait();
     PdlTrigger();
     const TPages &c = p.C;
-    const TSeqKeys keys = SeqTiles(p, seq);
-    if (slot < keys.First * PD_TILE || slot >= keys.End || keys.Count == 0) {
+    const TSeqKeys keys = SeqTiles<PD_RANGE_TILE>(p, seq);
+    if (slot < keys.First * PD_RANGE_TILE || slot >= keys.End || keys.Count == 0) {
         return;
     }
     const int page = c.Table.Row(seq)[slot >> c.PageShift];
@@ -716,23 +674,11 @@ static TPagedWorkspace PagedWorkspace(int headDim, int nSeq, int kvHeads, int he
     return w;
 }
 
-typedef void (*TPagedDecodeFn)(const TPagedDecodeParams);
-template <int D, bool E4M3, bool SCALE_F16, bool WIDE, bool TRACK>
-static TPagedDecodeFn PickSingle(bool single)
+template <int D, bool E4M3>
+static const void *PickCluster(bool f16, bool wide)
 {
-    return single ? PagedDecodeKernel<D, E4M3, SCALE_F16, WIDE, TRACK, true> : PagedDecodeKernel<D, E4M3, SCALE_F16, WIDE, TRACK, false>;
-}
-template <int D, bool E4M3, bool SCALE_F16>
-static TPagedDecodeFn PickWide(bool wide, bool track, bool single)
-{
-    return wide ? (track ? PickSingle<D, E4M3, SCALE_F16, true, true>(single) : PickSingle<D, E4M3, SCALE_F16, true, false>(single))
-                : (track ? PickSingle<D, E4M3, SCALE_F16, false, true>(single) : PickSingle<D, E4M3, SCALE_F16, false, false>(single));
-}
-template <int D>
-static TPagedDecodeFn PickTypes(bool e4m3, bool f16, bool wide, bool track, bool single)
-{
-    return e4m3 ? (f16 ? PickWide<D, true, true>(wide, track, single) : PickWide<D, true, false>(wide, track, single))
-                : (f16 ? PickWide<D, false, true>(wide, track, single) : PickWide<D, false, false>(wide, track, single));
+    return f16 ? (wide ? (const void *)PagedClusterKernel<D, E4M3, true, true> : (const void *)PagedClusterKernel<D, E4M3, true, false>)
+               : (wide ? (const void *)PagedClusterKernel<D, E4M3, false, true> : (const void *)PagedClusterKernel<D, E4M3, false, false>);
 }
 
 } // namespace tsa
@@ -804,35 +750,36 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     p.Out = P2D<char>(out);
     p.Partial = (float *)workspace;
     p.Lse = track ? (float *)((char *)workspace + ws.Lse) : nullptr;
-    p.Logits = (float *)((char *)workspace + ws.Logits);
+    p.Logits = track ? (float *)((char *)workspace + ws.Logits) : nullptr;
     p.LogitRow = ws.LogitRow;
     p.Status = statusWord;
-    const bool single = tilesMax <= PD_MIN_TILES + 1;
     const bool wide = p.Group > 8, e4m3 = cfg->kv_dtype == TSA_E4M3, f16 = cfg->scale_dtype == TSA_F16;
-    const void *kern = (const void *)(D == 128 ? PickTypes<128>(e4m3, f16, wide, track, single) : PickTypes<64>(e4m3, f16, wide, track, single));
-    int dev = 0, sms = 0, perSm = 0;
+    p.ScaleF16 = f16;
+    int dev = 0, sms = 0;
     rc = CheckCuda(cudaGetDevice(&dev), "cudaGetDevice");
     if (rc == TSA_OK) {
         rc = CheckCuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
     }
-    if (rc == TSA_OK) {
-        rc = CheckCuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&perSm, kern, PD_THREADS, 0), "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
-    }
     if (rc != TSA_OK) {
         return rc;
     }
-    long long grid = units;
-    if (!single) {
-        const long long resident = (long long)sms * (perSm < 1 ? 1 : perSm);
-        grid = (units * tilesMax + PD_MIN_TILES - 1) / PD_MIN_TILES;
-        grid = grid < resident ? grid : resident;
-        grid = grid < PD_MAX_CTAS ? grid : PD_MAX_CTAS;
-    }
     cudaStream_t s = (cudaStream_t)stream;
-    unsigned ctas = (unsigned)grid;
+    // clusters of CTAs of two to eight tiles per warp, while at most two CTAs come to an SM; units that share a key head's weights leave
+    // them to the second kernel of the ranges
+    p.Cluster = 1;
+    while (p.Cluster < PD_MAX_CLUSTER && tilesMax > (PD_MIN_TILES + 1) * p.Cluster) {
+        p.Cluster *= 2;
+    }
+    if ((p.Cluster == 1 || (tilesMax <= 4 * PD_MIN_TILES * p.Cluster && units * p.Cluster <= 2ll * sms)) && !(track && p.HeadChunks > 1)) {
+        const void *kern = D == 128 ? (e4m3 ? PickCluster<128, true>(f16, wide) : PickCluster<128, false>(f16, wide))
+                                    : (e4m3 ? PickCluster<64, true>(f16, wide) : PickCluster<64, false>(f16, wide));
+        void *args[] = {&p};
+        return CheckCuda(LaunchPdl(kern, dim3((unsigned)(units * p.Cluster)), dim3(PD_THREADS), 0, s, args, p.Cluster), "tsa_paged_decode launch");
+    }
+    unsigned ctas = 0;
+    rc = LaunchPagedRanges(p, kv, D, e4m3, keysMax / PD_RANGE_TILE + 2, &ctas, s);
     void *args[] = {&p, &ctas};
-    rc = CheckCuda(LaunchPdl(kern, dim3(ctas), dim3(PD_THREADS), 0, s, args), "tsa_paged_decode launch");
-    if (rc == TSA_OK && !single) {
+    if (rc == TSA_OK) {
         const void *join = D == 128 ? (const void *)PagedJoinKernel<128> : (const void *)PagedJoinKernel<64>;
         rc = CheckCuda(LaunchPdl(join, dim3(headCount, nSeq), dim3(128), 0, s, args), "tsa_paged_decode join launch");
     }
