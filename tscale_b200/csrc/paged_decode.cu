@@ -136,8 +136,8 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     const int unitsPerSeq = c.KvHeads * p.HeadChunks, ctas = p.Cluster, rank = blockIdx.x % ctas, unit = blockIdx.x / ctas;
     const int seq = unit / unitsPerSeq, head = unit % unitsPerSeq / p.HeadChunks, chunk = unit % p.HeadChunks;
     const int firstHead = head * p.Group + chunk * PD_ROWS, rows = min(p.Group - chunk * PD_ROWS, PD_ROWS);
-    PdlWait();
     PdlTrigger();
+    PdlWait();
     if (tid == 0 && p.Status && (p.CtxLens[seq] > p.MaxCtx || p.CtxLens[seq] > TableTokens(c))) {
         atomicOr(p.Status, kDevBadSpan);
     }
@@ -551,108 +551,227 @@ __device__ __forceinline__ void SeqStart(const TPagedDecodeParams &p, int seq, i
     *per = RangeTiles((unsigned)__reduce_add_sync(0xffffffffu, all) * units, ctas);
 }
 
-// Joins the partial sums of one (sequence, query head) in the order of the ranges, and adds the sink.  Heads that one range held are
-// finished already; sequences without keys get zeros.
+// Where the partial sums of a unit are: `chunks` of them, one behind the other by `stride` floats; 0: one range held the unit, which is done
+struct TPartials {
+    const float *Base;
+    size_t Stride;
+    int Chunks;
+};
 template <int D>
-__global__ void __launch_bounds__(128) PagedJoinKernel(const TPagedDecodeParams p, unsigned ctas)
+__device__ __forceinline__ TPartials UnitPartials(const TPagedDecodeParams &p, unsigned start, unsigned per, int count, int seq, int unit)
 {
-    constexpr int LPC = D / 4, GROUPS = 128 / LPC;
-    __shared__ float redMax[4];
-    __shared__ float sumL[GROUPS];
-    __shared__ float4 sumAcc[GROUPS][LPC];
-    const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
-    const int kvHead = head / p.Group, inGroup = head % p.Group, chunk = inGroup / PD_ROWS, row = inGroup % PD_ROWS;
-    const int inSeq = kvHead * p.HeadChunks + chunk;
-    unsigned start, per;
-    // the lengths were there before the kernel whose sums are joined began
-    SeqStart(p, seq, lane, ctas, &start, &per);
-    const int count = SeqTiles<PD_RANGE_TILE>(p, seq).Count;
-    PdlWait();
-    PdlTrigger();
-    if (count == 0) {
-        if (tid < D) {
-            StoreFromFloat(p.Out.Row(seq), head * D + tid, p.OutDtype, 0.0f);
-        }
-        if (p.Lse && tid == 0) {
-            p.Lse[(size_t)seq * p.HeadCount + head] = 0.0f;
-        }
-        return;
-    }
-    start += (unsigned)inSeq * count;
+    start += (unsigned)unit * count;
     const unsigned c0 = start / per, c1 = (start + count - 1) / per;
-    if (c0 == c1) {
-        return;
-    }
-    const int chunks = c1 - c0 + 1;
-    const size_t stride = (size_t)p.Rows * (D + 4);
-    const float *base = PartialRecord(p, D, c0, seq, inSeq, row);
-    float m = -60.0f;
-    for (int i = tid; i < chunks; i += 128) {
-        m = fmaxf(m, base[i * stride + D]);
-    }
-    m = WarpMax(m);
-    if (lane == 0) {
-        redMax[tid >> 5] = m;
-    }
-    __syncthreads();
-    m = fmaxf(fmaxf(redMax[0], redMax[1]), fmaxf(redMax[2], redMax[3]));
-    const int group = tid / LPC, sub = tid % LPC;
-    float l = 0;
-    float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-    for (int i = group; i < chunks; i += GROUPS) {
-        const float *src = base + i * stride;
-        const float2 ml = *reinterpret_cast<const float2 *>(src + D);
-        const float4 v = *reinterpret_cast<const float4 *>(src + 4 * sub);
-        const float f = Exp2(ml.x - m);
-        l = fmaf(f, ml.y, l);
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
-    }
-    sumAcc[group][sub] = acc;
-    if (sub == 0) {
-        sumL[group] = l;
-    }
-    __syncthreads();
-    if (tid < D) {
-        l = Exp2(-m);
-        float a = 0;
+    TPartials r;
+    r.Base = PartialRecord(p, D, c0, seq, unit, 0);
+    r.Stride = (size_t)p.Rows * (D + 4);
+    r.Chunks = c0 == c1 ? 0 : c1 - c0 + 1;
+    return r;
+}
+
+// records base + i * stride, i = first, first + step, ..: their sums of 4 dimensions (column 4 sub) and of the weights, relative to m
+template <int D>
+__device__ __forceinline__ void AddRecords(const float *base, size_t stride, int chunks, int first, int step, int sub, float &m, float &l, float4 &acc)
+{
+    for (int i = first; i < chunks; i += 4 * step) {
+        float2 ml[4];
+        float4 v[4];
+        float top = m;
 #pragma unroll
-        for (int i = 0; i < GROUPS; ++i) {
-            l += sumL[i];
-            a += reinterpret_cast<const float *>(sumAcc[i])[tid];
+        for (int j = 0; j < 4; ++j) { // four at a time are on their way
+            const bool in = i + j * step < chunks;
+            const float *src = base + (in ? i + j * step : i) * stride;
+            ml[j] = *reinterpret_cast<const float2 *>(src + D);
+            v[j] = *reinterpret_cast<const float4 *>(src + 4 * sub);
+            ml[j].x = in ? ml[j].x : -INFINITY;
         }
-        StoreFromFloat(p.Out.Row(seq), head * D + tid, p.OutDtype, a / l);
-        if (p.Lse && tid == 0) {
-            p.Lse[(size_t)seq * p.HeadCount + head] = m + Log2(l);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            top = fmaxf(top, ml[j].x);
+        }
+        const float f = Exp2(m - top);
+        m = top;
+        l *= f;
+        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i + j * step < chunks) {
+                const float w = Exp2(ml[j].x - m);
+                l = fmaf(w, ml[j].y, l);
+                acc = make_float4(fmaf(w, v[j].x, acc.x), fmaf(w, v[j].y, acc.y), fmaf(w, v[j].z, acc.z), fmaf(w, v[j].w, acc.w));
+            }
         }
     }
 }
 
-// weight[slot] += sum over the heads of a key head of 2^(z - lse): one thread per slot
-__global__ void __launch_bounds__(256) PagedWeightKernel(const TPagedDecodeParams p)
+// Behind the ranges.  The first joinCtas CTAs join the units that range borders cut, the records in the order of the ranges, and add the
+// sink.  Few units, many records of each (byUnit): a CTA has one row of one unit.  Otherwise CTA b has the unit that border b is the first
+// to cut, a group of D / 4 threads a row at a time.  They also write the zeros of sequences without keys.  The other CTAs (caches that keep
+// weights) have FIN_SLOTS slots of a key head: weight += sum over its query heads of 2^(z - log2 of all weights and the sink).
+constexpr int FIN_THREADS = 256, FIN_SLOTS = 4 * FIN_THREADS;
+template <int D>
+__global__ void __launch_bounds__(FIN_THREADS) PagedFinishKernel(const TPagedDecodeParams p, unsigned ctas, unsigned joinCtas, bool byUnit)
 {
-    const int head = blockIdx.y, seq = blockIdx.z, slot = blockIdx.x * 256 + threadIdx.x;
-    PdlWait();
+    constexpr int LPC = D / 4, GROUPS = FIN_THREADS / LPC, WARPS = FIN_THREADS / 32;
+    __shared__ float refOf[GROUPS], sumOf[GROUPS];
+    __shared__ float4 accOf[GROUPS][LPC];
+    __shared__ float lseOf[PD_ROWS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     PdlTrigger();
+    // the lengths were there before the kernel whose sums are joined began: all that follows from them is worked out before it ends
+    if (blockIdx.x < joinCtas) {
+        TSegment seg = {};
+        unsigned start, per;
+        int first = 0, chunks = 0; // records of the unit
+        if (byUnit) {
+            const int units = p.C.KvHeads * p.HeadChunks, unit = blockIdx.x / p.Rows;
+            seg.Seq = unit / units;
+            seg.Unit = unit % units;
+            SeqStart(p, seg.Seq, lane, ctas, &start, &per);
+            seg.Keys = SeqTiles<PD_RANGE_TILE>(p, seg.Seq);
+            if (seg.Keys.Count > 0) {
+                start += (unsigned)seg.Unit * seg.Keys.Count;
+                first = start / per;
+                chunks = (start + seg.Keys.Count - 1) / per - first + 1;
+                chunks = chunks > 1 ? chunks : 0;
+            }
+        } else if (blockIdx.x > 0) {
+            TRangeWalk walk;
+            if (walk.Begin(p, lane, blockIdx.x, ctas, false)) {
+                seg = walk.Segment(p);
+                start = walk.SeqBase + (unsigned)seg.Unit * seg.Keys.Count;
+                if (walk.At > start && walk.At - walk.Per <= start) {
+                    first = blockIdx.x - 1;
+                    chunks = (start + seg.Keys.Count - 1) / walk.Per - first + 1;
+                }
+            }
+        }
+        PdlWait();
+        for (int s = blockIdx.x; s < p.NSeq; s += joinCtas) {
+            if (SeqTiles<PD_RANGE_TILE>(p, s).Count == 0) {
+                for (int x = tid; x < p.HeadCount * D; x += FIN_THREADS) {
+                    StoreFromFloat(p.Out.Row(s), x, p.OutDtype, 0.0f);
+                }
+            }
+        }
+        if (chunks == 0) {
+            return;
+        }
+        const int group = tid / LPC, sub = tid % LPC;
+        const int firstHead = seg.Unit / p.HeadChunks * p.Group + seg.Unit % p.HeadChunks * PD_ROWS;
+        const int rows = min(p.Group - seg.Unit % p.HeadChunks * PD_ROWS, PD_ROWS);
+        const float *base = PartialRecord(p, D, first, seg.Seq, seg.Unit, 0);
+        const size_t stride = (size_t)p.Rows * (D + 4);
+        if (!byUnit) {
+            for (int r = group; r < rows; r += GROUPS) {
+                float m = -60.0f, l = 0;
+                float4 acc = make_float4(0, 0, 0, 0);
+                AddRecords<D>(base + r * (D + 4), stride, chunks, 0, 1, sub, m, l, acc);
+                l += Exp2(-m);
+                const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    StoreFromFloat(p.Out.Row(seg.Seq), (firstHead + r) * D + 4 * sub + i, p.OutDtype, v[i] / l);
+                }
+            }
+            return;
+        }
+        const int r = blockIdx.x % p.Rows;
+        if (r >= rows) {
+            return;
+        }
+        float m = -60.0f, l = 0;
+        float4 acc = make_float4(0, 0, 0, 0);
+        AddRecords<D>(base + r * (D + 4), stride, chunks, group, GROUPS, sub, m, l, acc);
+        accOf[group][sub] = acc;
+        if (sub == 0) {
+            refOf[group] = m;
+            sumOf[group] = l;
+        }
+        __syncthreads();
+        if (tid < D) {
+            m = refOf[0];
+#pragma unroll
+            for (int i = 1; i < GROUPS; ++i) {
+                m = fmaxf(m, refOf[i]);
+            }
+            l = Exp2(-m);
+            float a = 0;
+#pragma unroll
+            for (int i = 0; i < GROUPS; ++i) {
+                const float f = Exp2(refOf[i] - m);
+                l = fmaf(f, sumOf[i], l);
+                a = fmaf(f, reinterpret_cast<const float *>(accOf[i])[tid], a);
+            }
+            StoreFromFloat(p.Out.Row(seg.Seq), (firstHead + r) * D + tid, p.OutDtype, a / l);
+        }
+        return;
+    }
     const TPages &c = p.C;
+    const int slotParts = (min((long long)p.MaxCtx, TableTokens(c)) + FIN_SLOTS - 1) / FIN_SLOTS;
+    const int task = blockIdx.x - joinCtas, seq = task / (slotParts * c.KvHeads), kvHead = task / slotParts % c.KvHeads;
+    const int slot0 = task % slotParts * FIN_SLOTS, slot = slot0 + 4 * tid;
+    unsigned start, per;
+    SeqStart(p, seq, lane, ctas, &start, &per);
     const TSeqKeys keys = SeqTiles<PD_RANGE_TILE>(p, seq);
-    if (slot < keys.First * PD_RANGE_TILE || slot >= keys.End || keys.Count == 0) {
+    PdlWait();
+    if (slot0 >= keys.End || slot0 + FIN_SLOTS <= keys.First * PD_RANGE_TILE) {
         return;
     }
-    const int page = c.Table.Row(seq)[slot >> c.PageShift];
-    if ((unsigned)page >= (unsigned)c.PageCount) {
-        return;
+    const bool in = slot < keys.End && slot + 3 >= keys.First * PD_RANGE_TILE;
+    const int page = in ? c.Table.Row(seq)[slot >> c.PageShift] : -1;
+    float4 w = make_float4(0, 0, 0, 0);
+    for (int h0 = 0; h0 < p.Group; h0 += PD_ROWS) {
+        const int unit = kvHead * p.HeadChunks + h0 / PD_ROWS, rows = min(p.Group - h0, PD_ROWS), firstHead = kvHead * p.Group + h0;
+        const TPartials part = UnitPartials<D>(p, start, per, keys.Count, seq, unit);
+        __syncthreads(); // lseOf has been read
+        for (int r = warp; r < rows; r += WARPS) {
+            if (part.Chunks == 0) {
+                if (lane == 0) {
+                    lseOf[r] = p.Lse[(size_t)seq * p.HeadCount + firstHead + r];
+                }
+            } else {
+                const float *base = part.Base + r * (D + 4) + D;
+                float m = -60.0f;
+                for (int i = lane; i < part.Chunks; i += 32) {
+                    m = fmaxf(m, base[i * part.Stride]);
+                }
+                m = WarpMax(m);
+                float l = 0;
+                for (int i = lane; i < part.Chunks; i += 32) {
+                    l = fmaf(Exp2(base[i * part.Stride] - m), base[i * part.Stride + 1], l);
+                }
+                l = WarpSum(l) + Exp2(-m);
+                if (lane == 0) {
+                    lseOf[r] = m + Log2(l);
+                }
+            }
+        }
+        __syncthreads();
+        if (in) {
+            const float *z = p.Logits + ((size_t)seq * p.HeadCount + firstHead) * p.LogitRow + slot;
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) {
+                const float4 x = *reinterpret_cast<const float4 *>(z + (size_t)r * p.LogitRow);
+                const float lse = lseOf[r];
+                w.x += Exp2(x.x - lse);
+                w.y += Exp2(x.y - lse);
+                w.z += Exp2(x.z - lse);
+                w.w += Exp2(x.w - lse);
+            }
+        }
     }
-    const float *lse = p.Lse + (size_t)seq * p.HeadCount + head * p.Group;
-    const float *z = p.Logits + ((size_t)seq * p.HeadCount + head * p.Group) * p.LogitRow + slot;
-    float w = 0;
-    for (int i = 0; i < p.Group; ++i) {
-        w += Exp2(z[(size_t)i * p.LogitRow] - lse[i]);
+    if ((unsigned)page < (unsigned)c.PageCount) {
+        float *dst = c.Weight + PlaneSlot(c, page, kvHead) + (slot & ((1 << c.PageShift) - 1));
+        float4 old = *reinterpret_cast<const float4 *>(dst);
+        // slots that the ranges did not look at have no logits
+        const int first = keys.First * PD_RANGE_TILE;
+        old.x += slot >= first && slot < keys.End ? w.x : 0.0f;
+        old.y += slot + 1 >= first && slot + 1 < keys.End ? w.y : 0.0f;
+        old.z += slot + 2 >= first && slot + 2 < keys.End ? w.z : 0.0f;
+        old.w += slot + 3 >= first && slot + 3 < keys.End ? w.w : 0.0f;
+        *reinterpret_cast<float4 *>(dst) = old;
     }
-    c.Weight[PlaneSlot(c, page, head) + (slot & ((1 << c.PageShift) - 1))] += w;
 }
 
 // parts of the workspace, in this order
@@ -778,14 +897,14 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     }
     unsigned ctas = 0;
     rc = LaunchPagedRanges(p, kv, D, e4m3, keysMax / PD_RANGE_TILE + 2, &ctas, s);
-    void *args[] = {&p, &ctas};
     if (rc == TSA_OK) {
-        const void *join = D == 128 ? (const void *)PagedJoinKernel<128> : (const void *)PagedJoinKernel<64>;
-        rc = CheckCuda(LaunchPdl(join, dim3(headCount, nSeq), dim3(128), 0, s, args), "tsa_paged_decode join launch");
-    }
-    if (rc == TSA_OK && track && longest > 0) {
-        rc = CheckCuda(LaunchPdl((const void *)PagedWeightKernel, dim3((longest + 255) / 256, kv->kv_heads, nSeq), dim3(256), 0, s, args),
-            "tsa_paged_decode weights launch");
+        const void *finish = D == 128 ? (const void *)PagedFinishKernel<128> : (const void *)PagedFinishKernel<64>;
+        bool byUnit = units * 4 < ctas;
+        unsigned joinCtas = byUnit ? (unsigned)units * p.Rows : ctas;
+        const long long weightCtas = track ? (long long)((longest + FIN_SLOTS - 1) / FIN_SLOTS) * kv->kv_heads * nSeq : 0;
+        TSA_REQUIRE(weightCtas < (1ll << 30), "tsa_paged_decode: %d sequences of %d tokens with weights are too much for one call", nSeq, longest);
+        void *args[] = {&p, &ctas, &joinCtas, &byUnit};
+        rc = CheckCuda(LaunchPdl(finish, dim3((unsigned)(joinCtas + weightCtas)), dim3(FIN_THREADS), 0, s, args), "tsa_paged_decode join launch");
     }
     return rc;
 }

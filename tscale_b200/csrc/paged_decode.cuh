@@ -87,7 +87,7 @@ struct TSegment {
 
 // The segments of a range.  A whole warp calls these; every lane has the same answers.
 struct TRangeWalk {
-    unsigned At, End, SeqBase;
+    unsigned At, End, SeqBase, Per;
     int Seq, UnitsPerSeq;
 
     // false: the range is empty; report: sequences that do not fit set the status word
@@ -102,9 +102,9 @@ struct TRangeWalk {
             }
         }
         const unsigned total = (unsigned)__reduce_add_sync(0xffffffffu, sum) * UnitsPerSeq;
-        const unsigned per = RangeTiles(total, ctas);
-        At = cta * per;
-        End = min(At + per, total);
+        Per = RangeTiles(total, ctas);
+        At = cta * Per;
+        End = min(At + Per, total);
         if (At >= End) {
             return false;
         }

@@ -34,7 +34,8 @@ struct TTileKeys {
 template <int D, int HB>
 struct TTcLayout {
     static constexpr int TILE_BYTES = PT_KEYS * D;
-    static constexpr int STAGES = D == 128 ? 3 : 5; // of the ring of K and V tiles
+    static constexpr int CTAS = D == 64 && HB < 4 ? 3 : 2; // per SM
+    static constexpr int STAGES = D == 64 && HB == 4 ? 5 : 3; // of the ring of K and V tiles
     static constexpr int RING_BYTES = STAGES * 2 * TILE_BYTES;
     static constexpr int Q_BYTES = PD_ROWS * D;
     static constexpr int W_BYTES = HB * PT_KEYS * 16;
@@ -122,7 +123,7 @@ __device__ __forceinline__ void WarpSums(float (&v)[N], int lane)
 
 // HB: blocks of four query heads (1, 2 or 4)
 template <int D, bool E4M3, int HB>
-__global__ void __launch_bounds__(PT_THREADS, 2) PagedRangeKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+__global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRangeKernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
     const TPagedDecodeParams p)
 {
     typedef TTcLayout<D, HB> TL;
@@ -643,17 +644,20 @@ __global__ void __launch_bounds__(PT_THREADS, 2) PagedRangeKernel(const __grid_c
 }
 
 template <int D, bool E4M3>
-static const void *PickBlocks(int rows, size_t *smem)
+static const void *PickBlocks(int rows, size_t *smem, int *perSm)
 {
     if (rows <= 4) {
         *smem = TTcLayout<D, 1>::BYTES;
+        *perSm = TTcLayout<D, 1>::CTAS;
         return (const void *)PagedRangeKernel<D, E4M3, 1>;
     }
     if (rows <= 8) {
         *smem = TTcLayout<D, 2>::BYTES;
+        *perSm = TTcLayout<D, 2>::CTAS;
         return (const void *)PagedRangeKernel<D, E4M3, 2>;
     }
     *smem = TTcLayout<D, 4>::BYTES;
+    *perSm = TTcLayout<D, 4>::CTAS;
     return (const void *)PagedRangeKernel<D, E4M3, 4>;
 }
 
@@ -674,8 +678,9 @@ int LaunchPagedRanges(const TPagedDecodeParams &p, const tsa_paged_kv *kv, int h
         return rc;
     }
     size_t smem = 0;
-    const void *kern = headDim == 128 ? (e4m3 ? PickBlocks<128, true>(p.Rows, &smem) : PickBlocks<128, false>(p.Rows, &smem))
-                                      : (e4m3 ? PickBlocks<64, true>(p.Rows, &smem) : PickBlocks<64, false>(p.Rows, &smem));
+    int perSm = 0;
+    const void *kern = headDim == 128 ? (e4m3 ? PickBlocks<128, true>(p.Rows, &smem, &perSm) : PickBlocks<128, false>(p.Rows, &smem, &perSm))
+                                      : (e4m3 ? PickBlocks<64, true>(p.Rows, &smem, &perSm) : PickBlocks<64, false>(p.Rows, &smem, &perSm));
     int dev = 0, sms = 0;
     rc = CheckCuda(cudaGetDevice(&dev), "cudaGetDevice");
     if (rc == TSA_OK) {
@@ -688,7 +693,7 @@ int LaunchPagedRanges(const TPagedDecodeParams &p, const tsa_paged_kv *kv, int h
         return rc;
     }
     const long long total = tilesMax * p.NSeq * kv->kv_heads * p.HeadChunks;
-    *ctas = (unsigned)(total < 2 * sms ? total : 2 * sms);
+    *ctas = (unsigned)(total < perSm * sms ? total : perSm * sms);
     *ctas = *ctas < PD_MAX_CTAS ? *ctas : PD_MAX_CTAS;
     TPagedDecodeParams copy = p;
     void *args[] = {&tmK, &tmV, &copy};
