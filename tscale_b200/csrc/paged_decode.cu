@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     constexpr int ROWS = 8 * HALVES;
     typedef typename std::conditional<D == 128, uint4, uint2>::type TPiece; // D / 8 dimensions of a key
     __shared__ __align__(16) float accOf[PD_WARPS][ROWS][D + 4]; // [.][.][16 j + 2 g + b] for dimension D / 8 g + 2 j + b: no two lanes of a store meet in a bank
-    __shared__ float refOf[PD_WARPS][ROWS], sumOf[PD_WARPS][ROWS], lseOf[ROWS];
+    __shared__ float refOf[PD_WARPS][ROWS], sumOf[PD_WARPS][ROWS], ctaRef[ROWS], ctaSum[ROWS], lseOf[ROWS], factorOf[ROWS][PD_MAX_CLUSTER];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const TPages &c = p.C;
     const int unitsPerSeq = c.KvHeads * p.HeadChunks, ctas = p.Cluster, rank = blockIdx.x % ctas, unit = blockIdx.x / ctas;
@@ -478,53 +478,93 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
             }
         }
     }
+    __syncthreads();
+    // the CTA's sums: in the place of its first warp's
+    for (int x = tid; x < rows * D; x += PD_THREADS) {
+        const int r = x / D, i = x % D;
+        float m = refOf[0][r];
+#pragma unroll
+        for (int w = 1; w < PD_WARPS; ++w) {
+            m = fmaxf(m, refOf[w][r]);
+        }
+        float a = 0;
+#pragma unroll
+        for (int w = 0; w < PD_WARPS; ++w) {
+            a = fmaf(Exp2(refOf[w][r] - m), accOf[w][r][i], a);
+        }
+        accOf[0][r][i] = a;
+    }
+    if (tid < rows) {
+        float m = refOf[0][tid], s = 0;
+#pragma unroll
+        for (int w = 1; w < PD_WARPS; ++w) {
+            m = fmaxf(m, refOf[w][tid]);
+        }
+#pragma unroll
+        for (int w = 0; w < PD_WARPS; ++w) {
+            s = fmaf(Exp2(refOf[w][tid] - m), sumOf[w][tid], s);
+        }
+        ctaRef[tid] = m;
+        ctaSum[tid] = s;
+    }
     if (ctas > 1) {
-        // each CTA of the cluster finishes a part of the result from all their sums
         ClusterSync();
     } else {
         __syncthreads();
     }
-    auto refAt = [&](int i, int r) { return ctas > 1 ? ClusterLoad(&refOf[i % PD_WARPS][r], i / PD_WARPS) : refOf[i][r]; };
-    auto sumAt = [&](int i, int r) { return ctas > 1 ? ClusterLoad(&sumOf[i % PD_WARPS][r], i / PD_WARPS) : sumOf[i][r]; };
-    auto accAt = [&](int i, int r, int x) { return ctas > 1 ? ClusterLoad(&accOf[i % PD_WARPS][r][x], i / PD_WARPS) : accOf[i][r][x]; };
-    // reference of all warps' sums of row r (at least -60: then the sink, weight 1 at logit 0, stays in range) and their weights' sum
-    auto joined = [&](int r, float *sumAll) {
-        float m = -60.0f;
-#pragma unroll 4
-        for (int w = 0; w < PD_WARPS * ctas; ++w) {
-            m = fmaxf(m, refAt(w, r));
+    // every CTA of the cluster finishes a part of the result from all their sums: eight threads per row find the factors of the CTAs' sums.
+    // The reference is at least -60: the sink, weight 1 at logit 0, then stays in range
+    static_assert(PD_MAX_CLUSTER == 8 && 8 * PD_ROWS <= PD_THREADS, "a thread per row and CTA");
+    {
+        const int r = tid >> 3, i = tid & 7;
+        const bool in = r < rows && i < ctas;
+        const float ref1 = in ? ClusterLoad(&ctaRef[r], i) : PD_NO_REF, sum1 = in ? ClusterLoad(&ctaSum[r], i) : 0.0f;
+        float m = fmaxf(ref1, -60.0f);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         }
-        float s = Exp2(-m);
-#pragma unroll 4
-        for (int w = 0; w < PD_WARPS * ctas; ++w) {
-            s = fmaf(Exp2(refAt(w, r) - m), sumAt(w, r), s);
+        const float f = Exp2(ref1 - m);
+        float s = f * sum1;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
         }
-        *sumAll = s;
-        return m;
-    };
+        s += Exp2(-m);
+        if (r < rows) {
+            factorOf[r][i] = f / s;
+            if (i == 0) {
+                lseOf[r] = m + Log2(s);
+            }
+        }
+    }
+    __syncthreads();
     for (int x = rank * PD_THREADS + tid; x < rows * D; x += ctas * PD_THREADS) {
         const int r = x / D, i = x % D;
         const int d = (i >> 1 & 7) * (D / 8) + 2 * (i >> 4) + (i & 1);
-        float s, a = 0;
-        const float m = joined(r, &s);
-#pragma unroll 4
-        for (int w = 0; w < PD_WARPS * ctas; ++w) {
-            a = fmaf(Exp2(refAt(w, r) - m), accAt(w, r, i), a);
+        float a = 0;
+        if (ctas == 1) {
+            a = factorOf[r][0] * accOf[0][r][i];
+        } else {
+            float accs[PD_MAX_CLUSTER];
+#pragma unroll
+            for (int j = 0; j < PD_MAX_CLUSTER; ++j) {
+                accs[j] = j < ctas ? ClusterLoad(&accOf[0][r][i], j) : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < PD_MAX_CLUSTER; ++j) {
+                a = j < ctas ? fmaf(factorOf[r][j], accs[j], a) : a;
+            }
         }
-        StoreFromFloat(p.Out.Row(seq), (firstHead + r) * D + d, p.OutDtype, a / s);
+        StoreFromFloat(p.Out.Row(seq), (firstHead + r) * D + d, p.OutDtype, a);
     }
     if (logits) {
         // the weights of this CTA's keys (one unit per key head: nobody else adds to them)
-        if (tid < rows) {
-            float s;
-            const float m = joined(tid, &s);
-            lseOf[tid] = m + Log2(s);
-        }
-        __syncthreads();
         for (int key = max(keyBeg, segBeg * PD_TILE) + tid; key < keyEnd; key += PD_THREADS) {
             const int page = table[key >> c.PageShift];
             if ((unsigned)page < (unsigned)c.PageCount) {
                 float w = 0;
+#pragma unroll 4
                 for (int r = 0; r < rows; ++r) {
                     w += Exp2(logits[(size_t)r * p.LogitRow + key] - lseOf[r]);
                 }
@@ -549,24 +589,6 @@ __device__ __forceinline__ void SeqStart(const TPagedDecodeParams &p, int seq, i
     const int units = p.C.KvHeads * p.HeadChunks;
     *start = (unsigned)__reduce_add_sync(0xffffffffu, before) * units;
     *per = RangeTiles((unsigned)__reduce_add_sync(0xffffffffu, all) * units, ctas);
-}
-
-// Where the partial sums of a unit are: `chunks` of them, one behind the other by `stride` floats; 0: one range held the unit, which is done
-struct TPartials {
-    const float *Base;
-    size_t Stride;
-    int Chunks;
-};
-template <int D>
-__device__ __forceinline__ TPartials UnitPartials(const TPagedDecodeParams &p, unsigned start, unsigned per, int count, int seq, int unit)
-{
-    start += (unsigned)unit * count;
-    const unsigned c0 = start / per, c1 = (start + count - 1) / per;
-    TPartials r;
-    r.Base = PartialRecord(p, D, c0, seq, unit, 0);
-    r.Stride = (size_t)p.Rows * (D + 4);
-    r.Chunks = c0 == c1 ? 0 : c1 - c0 + 1;
-    return r;
 }
 
 // records base + i * stride, i = first, first + step, ..: their sums of 4 dimensions (column 4 sub) and of the weights, relative to m
@@ -604,174 +626,152 @@ __device__ __forceinline__ void AddRecords(const float *base, size_t stride, int
     }
 }
 
-// Behind the ranges.  The first joinCtas CTAs join the units that range borders cut, the records in the order of the ranges, and add the
-// sink.  Few units, many records of each (byUnit): a CTA has one row of one unit.  Otherwise CTA b has the unit that border b is the first
-// to cut, a group of D / 4 threads a row at a time.  They also write the zeros of sequences without keys.  The other CTAs (caches that keep
-// weights) have FIN_SLOTS slots of a key head: weight += sum over its query heads of 2^(z - log2 of all weights and the sink).
-constexpr int FIN_THREADS = 256, FIN_SLOTS = 4 * FIN_THREADS;
+// Behind the ranges: joins the units that range borders cut, the records in the order of the ranges, and adds the sink.  Few units, many
+// records of each (byUnit): a CTA has one row of one unit.  Otherwise CTA b has the unit that border b is the first to cut, a group of
+// D / 4 threads a row at a time.  Also writes the zeros of sequences without keys.
+constexpr int FIN_THREADS = 256;
 template <int D>
-__global__ void __launch_bounds__(FIN_THREADS) PagedFinishKernel(const TPagedDecodeParams p, unsigned ctas, unsigned joinCtas, bool byUnit)
+__global__ void __launch_bounds__(FIN_THREADS) PagedJoinKernel(const TPagedDecodeParams p, unsigned ctas, bool byUnit)
 {
-    constexpr int LPC = D / 4, GROUPS = FIN_THREADS / LPC, WARPS = FIN_THREADS / 32;
+    constexpr int LPC = D / 4, GROUPS = FIN_THREADS / LPC;
     __shared__ float refOf[GROUPS], sumOf[GROUPS];
     __shared__ float4 accOf[GROUPS][LPC];
-    __shared__ float lseOf[PD_ROWS];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31;
     PdlTrigger();
     // the lengths were there before the kernel whose sums are joined began: all that follows from them is worked out before it ends
-    if (blockIdx.x < joinCtas) {
-        TSegment seg = {};
-        unsigned start, per;
-        int first = 0, chunks = 0; // records of the unit
-        if (byUnit) {
-            const int units = p.C.KvHeads * p.HeadChunks, unit = blockIdx.x / p.Rows;
-            seg.Seq = unit / units;
-            seg.Unit = unit % units;
-            SeqStart(p, seg.Seq, lane, ctas, &start, &per);
-            seg.Keys = SeqTiles<PD_RANGE_TILE>(p, seg.Seq);
-            if (seg.Keys.Count > 0) {
-                start += (unsigned)seg.Unit * seg.Keys.Count;
-                first = start / per;
-                chunks = (start + seg.Keys.Count - 1) / per - first + 1;
-                chunks = chunks > 1 ? chunks : 0;
-            }
-        } else if (blockIdx.x > 0) {
-            TRangeWalk walk;
-            if (walk.Begin(p, lane, blockIdx.x, ctas, false)) {
-                seg = walk.Segment(p);
-                start = walk.SeqBase + (unsigned)seg.Unit * seg.Keys.Count;
-                if (walk.At > start && walk.At - walk.Per <= start) {
-                    first = blockIdx.x - 1;
-                    chunks = (start + seg.Keys.Count - 1) / walk.Per - first + 1;
-                }
-            }
-        }
-        PdlWait();
-        for (int s = blockIdx.x; s < p.NSeq; s += joinCtas) {
-            if (SeqTiles<PD_RANGE_TILE>(p, s).Count == 0) {
-                for (int x = tid; x < p.HeadCount * D; x += FIN_THREADS) {
-                    StoreFromFloat(p.Out.Row(s), x, p.OutDtype, 0.0f);
-                }
-            }
-        }
-        if (chunks == 0) {
-            return;
-        }
-        const int group = tid / LPC, sub = tid % LPC;
-        const int firstHead = seg.Unit / p.HeadChunks * p.Group + seg.Unit % p.HeadChunks * PD_ROWS;
-        const int rows = min(p.Group - seg.Unit % p.HeadChunks * PD_ROWS, PD_ROWS);
-        const float *base = PartialRecord(p, D, first, seg.Seq, seg.Unit, 0);
-        const size_t stride = (size_t)p.Rows * (D + 4);
-        if (!byUnit) {
-            for (int r = group; r < rows; r += GROUPS) {
-                float m = -60.0f, l = 0;
-                float4 acc = make_float4(0, 0, 0, 0);
-                AddRecords<D>(base + r * (D + 4), stride, chunks, 0, 1, sub, m, l, acc);
-                l += Exp2(-m);
-                const float v[4] = {acc.x, acc.y, acc.z, acc.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    StoreFromFloat(p.Out.Row(seg.Seq), (firstHead + r) * D + 4 * sub + i, p.OutDtype, v[i] / l);
-                }
-            }
-            return;
-        }
-        const int r = blockIdx.x % p.Rows;
-        if (r >= rows) {
-            return;
-        }
-        float m = -60.0f, l = 0;
-        float4 acc = make_float4(0, 0, 0, 0);
-        AddRecords<D>(base + r * (D + 4), stride, chunks, group, GROUPS, sub, m, l, acc);
-        accOf[group][sub] = acc;
-        if (sub == 0) {
-            refOf[group] = m;
-            sumOf[group] = l;
-        }
-        __syncthreads();
-        if (tid < D) {
-            m = refOf[0];
-#pragma unroll
-            for (int i = 1; i < GROUPS; ++i) {
-                m = fmaxf(m, refOf[i]);
-            }
-            l = Exp2(-m);
-            float a = 0;
-#pragma unroll
-            for (int i = 0; i < GROUPS; ++i) {
-                const float f = Exp2(refOf[i] - m);
-                l = fmaf(f, sumOf[i], l);
-                a = fmaf(f, reinterpret_cast<const float *>(accOf[i])[tid], a);
-            }
-            StoreFromFloat(p.Out.Row(seg.Seq), (firstHead + r) * D + tid, p.OutDtype, a / l);
-        }
-        return;
-    }
-    const TPages &c = p.C;
-    const int slotParts = (min((long long)p.MaxCtx, TableTokens(c)) + FIN_SLOTS - 1) / FIN_SLOTS;
-    const int task = blockIdx.x - joinCtas, seq = task / (slotParts * c.KvHeads), kvHead = task / slotParts % c.KvHeads;
-    const int slot0 = task % slotParts * FIN_SLOTS, slot = slot0 + 4 * tid;
+    TSegment seg = {};
     unsigned start, per;
-    SeqStart(p, seq, lane, ctas, &start, &per);
-    const TSeqKeys keys = SeqTiles<PD_RANGE_TILE>(p, seq);
+    int first = 0, chunks = 0; // records of the unit
+    if (byUnit) {
+        const int units = p.C.KvHeads * p.HeadChunks, unit = blockIdx.x / p.Rows;
+        seg.Seq = unit / units;
+        seg.Unit = unit % units;
+        SeqStart(p, seg.Seq, lane, ctas, &start, &per);
+        seg.Keys = SeqTiles<PD_RANGE_TILE>(p, seg.Seq);
+        if (seg.Keys.Count > 0) {
+            start += (unsigned)seg.Unit * seg.Keys.Count;
+            first = start / per;
+            chunks = (start + seg.Keys.Count - 1) / per - first + 1;
+            chunks = chunks > 1 ? chunks : 0;
+        }
+    } else if (blockIdx.x > 0) {
+        TRangeWalk walk;
+        if (walk.Begin(p, lane, blockIdx.x, ctas, false)) {
+            seg = walk.Segment(p);
+            start = walk.SeqBase + (unsigned)seg.Unit * seg.Keys.Count;
+            if (walk.At > start && walk.At - walk.Per <= start) {
+                first = blockIdx.x - 1;
+                chunks = (start + seg.Keys.Count - 1) / walk.Per - first + 1;
+            }
+        }
+    }
     PdlWait();
-    if (slot0 >= keys.End || slot0 + FIN_SLOTS <= keys.First * PD_RANGE_TILE) {
+    for (int s = blockIdx.x; s < p.NSeq; s += gridDim.x) {
+        if (SeqTiles<PD_RANGE_TILE>(p, s).Count == 0) {
+            for (int x = tid; x < p.HeadCount * D; x += FIN_THREADS) {
+                StoreFromFloat(p.Out.Row(s), x, p.OutDtype, 0.0f);
+            }
+        }
+    }
+    if (chunks == 0) {
         return;
     }
-    const bool in = slot < keys.End && slot + 3 >= keys.First * PD_RANGE_TILE;
-    const int page = in ? c.Table.Row(seq)[slot >> c.PageShift] : -1;
+    const int group = tid / LPC, sub = tid % LPC;
+    const int firstHead = seg.Unit / p.HeadChunks * p.Group + seg.Unit % p.HeadChunks * PD_ROWS;
+    const int rows = min(p.Group - seg.Unit % p.HeadChunks * PD_ROWS, PD_ROWS);
+    const float *base = PartialRecord(p, D, first, seg.Seq, seg.Unit, 0);
+    const size_t stride = (size_t)p.Rows * (D + 4);
+    if (!byUnit) {
+        for (int r = group; r < rows; r += GROUPS) {
+            float m = -60.0f, l = 0;
+            float4 acc = make_float4(0, 0, 0, 0);
+            AddRecords<D>(base + r * (D + 4), stride, chunks, 0, 1, sub, m, l, acc);
+            l += Exp2(-m);
+            const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                StoreFromFloat(p.Out.Row(seg.Seq), (firstHead + r) * D + 4 * sub + i, p.OutDtype, v[i] / l);
+            }
+            if (p.Lse && sub == 0) {
+                p.Lse[(size_t)seg.Seq * p.HeadCount + firstHead + r] = m + Log2(l);
+            }
+        }
+        return;
+    }
+    const int r = blockIdx.x % p.Rows;
+    if (r >= rows) {
+        return;
+    }
+    float m = -60.0f, l = 0;
+    float4 acc = make_float4(0, 0, 0, 0);
+    AddRecords<D>(base + r * (D + 4), stride, chunks, group, GROUPS, sub, m, l, acc);
+    accOf[group][sub] = acc;
+    if (sub == 0) {
+        refOf[group] = m;
+        sumOf[group] = l;
+    }
+    __syncthreads();
+    if (tid < D) {
+        m = refOf[0];
+#pragma unroll
+        for (int i = 1; i < GROUPS; ++i) {
+            m = fmaxf(m, refOf[i]);
+        }
+        l = Exp2(-m);
+        float a = 0;
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            const float f = Exp2(refOf[i] - m);
+            l = fmaf(f, sumOf[i], l);
+            a = fmaf(f, reinterpret_cast<const float *>(accOf[i])[tid], a);
+        }
+        StoreFromFloat(p.Out.Row(seg.Seq), (firstHead + r) * D + tid, p.OutDtype, a / l);
+        if (p.Lse && tid == 0) {
+            p.Lse[(size_t)seg.Seq * p.HeadCount + firstHead + r] = m + Log2(l);
+        }
+    }
+}
+
+// weight += sum over the query heads of a key head of 2^(z - log2 of all weights and the sink): four slots per thread.  What does not come
+// from the kernels before (the lengths, the table, the weights, which only this kernel writes) is loaded before they end.
+constexpr int WGT_THREADS = 256, WGT_SLOTS = 4 * WGT_THREADS;
+__global__ void __launch_bounds__(WGT_THREADS) PagedWeightKernel(const TPagedDecodeParams p)
+{
+    const TPages &c = p.C;
+    const int kvHead = blockIdx.y, seq = blockIdx.z, slot = blockIdx.x * WGT_SLOTS + 4 * threadIdx.x;
+    PdlTrigger();
+    const TSeqKeys keys = SeqTiles<PD_RANGE_TILE>(p, seq);
+    const int first = keys.First * PD_RANGE_TILE; // slots that the ranges did not look at have no logits
+    const int page = slot < keys.End && slot + 3 >= first ? c.Table.Row(seq)[slot >> c.PageShift] : -1;
+    const bool in = (unsigned)page < (unsigned)c.PageCount;
+    float *const dst = c.Weight + PlaneSlot(c, in ? page : 0, kvHead) + (slot & ((1 << c.PageShift) - 1));
     float4 w = make_float4(0, 0, 0, 0);
-    for (int h0 = 0; h0 < p.Group; h0 += PD_ROWS) {
-        const int unit = kvHead * p.HeadChunks + h0 / PD_ROWS, rows = min(p.Group - h0, PD_ROWS), firstHead = kvHead * p.Group + h0;
-        const TPartials part = UnitPartials<D>(p, start, per, keys.Count, seq, unit);
-        __syncthreads(); // lseOf has been read
-        for (int r = warp; r < rows; r += WARPS) {
-            if (part.Chunks == 0) {
-                if (lane == 0) {
-                    lseOf[r] = p.Lse[(size_t)seq * p.HeadCount + firstHead + r];
-                }
-            } else {
-                const float *base = part.Base + r * (D + 4) + D;
-                float m = -60.0f;
-                for (int i = lane; i < part.Chunks; i += 32) {
-                    m = fmaxf(m, base[i * part.Stride]);
-                }
-                m = WarpMax(m);
-                float l = 0;
-                for (int i = lane; i < part.Chunks; i += 32) {
-                    l = fmaf(Exp2(base[i * part.Stride] - m), base[i * part.Stride + 1], l);
-                }
-                l = WarpSum(l) + Exp2(-m);
-                if (lane == 0) {
-                    lseOf[r] = m + Log2(l);
-                }
-            }
-        }
-        __syncthreads();
-        if (in) {
-            const float *z = p.Logits + ((size_t)seq * p.HeadCount + firstHead) * p.LogitRow + slot;
+    if (in) {
+        w = *reinterpret_cast<const float4 *>(dst);
+    }
+    PdlWait();
+    if (!in) {
+        return;
+    }
+    const size_t head = (size_t)seq * p.HeadCount + kvHead * p.Group;
+    const float *lse = p.Lse + head, *z = p.Logits + head * p.LogitRow + slot;
+    const bool whole = slot >= first && slot + 3 < keys.End;
 #pragma unroll 4
-            for (int r = 0; r < rows; ++r) {
-                const float4 x = *reinterpret_cast<const float4 *>(z + (size_t)r * p.LogitRow);
-                const float lse = lseOf[r];
-                w.x += Exp2(x.x - lse);
-                w.y += Exp2(x.y - lse);
-                w.z += Exp2(x.z - lse);
-                w.w += Exp2(x.w - lse);
-            }
+    for (int r = 0; r < p.Group; ++r) {
+        float4 x = *reinterpret_cast<const float4 *>(z + (size_t)r * p.LogitRow);
+        const float l = lse[r];
+        if (!whole) {
+            x.x = slot >= first && slot < keys.End ? x.x : -INFINITY;
+            x.y = slot + 1 >= first && slot + 1 < keys.End ? x.y : -INFINITY;
+            x.z = slot + 2 >= first && slot + 2 < keys.End ? x.z : -INFINITY;
+            x.w = slot + 3 >= first && slot + 3 < keys.End ? x.w : -INFINITY;
         }
+        w.x += Exp2(x.x - l);
+        w.y += Exp2(x.y - l);
+        w.z += Exp2(x.z - l);
+        w.w += Exp2(x.w - l);
     }
-    if ((unsigned)page < (unsigned)c.PageCount) {
-        float *dst = c.Weight + PlaneSlot(c, page, kvHead) + (slot & ((1 << c.PageShift) - 1));
-        float4 old = *reinterpret_cast<const float4 *>(dst);
-        // slots that the ranges did not look at have no logits
-        const int first = keys.First * PD_RANGE_TILE;
-        old.x += slot >= first && slot < keys.End ? w.x : 0.0f;
-        old.y += slot + 1 >= first && slot + 1 < keys.End ? w.y : 0.0f;
-        old.z += slot + 2 >= first && slot + 2 < keys.End ? w.z : 0.0f;
-        old.w += slot + 3 >= first && slot + 3 < keys.End ? w.w : 0.0f;
-        *reinterpret_cast<float4 *>(dst) = old;
-    }
+    *reinterpret_cast<float4 *>(dst) = w;
 }
 
 // parts of the workspace, in this order
@@ -898,13 +898,15 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     unsigned ctas = 0;
     rc = LaunchPagedRanges(p, kv, D, e4m3, keysMax / PD_RANGE_TILE + 2, &ctas, s);
     if (rc == TSA_OK) {
-        const void *finish = D == 128 ? (const void *)PagedFinishKernel<128> : (const void *)PagedFinishKernel<64>;
+        const void *join = D == 128 ? (const void *)PagedJoinKernel<128> : (const void *)PagedJoinKernel<64>;
         bool byUnit = units * 4 < ctas;
-        unsigned joinCtas = byUnit ? (unsigned)units * p.Rows : ctas;
-        const long long weightCtas = track ? (long long)((longest + FIN_SLOTS - 1) / FIN_SLOTS) * kv->kv_heads * nSeq : 0;
-        TSA_REQUIRE(weightCtas < (1ll << 30), "tsa_paged_decode: %d sequences of %d tokens with weights are too much for one call", nSeq, longest);
-        void *args[] = {&p, &ctas, &joinCtas, &byUnit};
-        rc = CheckCuda(LaunchPdl(finish, dim3((unsigned)(joinCtas + weightCtas)), dim3(FIN_THREADS), 0, s, args), "tsa_paged_decode join launch");
+        void *args[] = {&p, &ctas, &byUnit};
+        rc = CheckCuda(LaunchPdl(join, dim3(byUnit ? (unsigned)units * p.Rows : ctas), dim3(FIN_THREADS), 0, s, args), "tsa_paged_decode join launch");
+    }
+    if (rc == TSA_OK && track && longest > 0) {
+        void *args[] = {&p};
+        rc = CheckCuda(LaunchPdl((const void *)PagedWeightKernel, dim3((longest + WGT_SLOTS - 1) / WGT_SLOTS, kv->kv_heads, nSeq), dim3(WGT_THREADS), 0, s, args),
+            "tsa_paged_decode weights launch");
     }
     return rc;
 }
