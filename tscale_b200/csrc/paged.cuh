@@ -27,9 +27,18 @@ __host__ __device__ __forceinline__ long long TableTokens(const TPages &c)
     return (long long)c.TableCols << c.PageShift;
 }
 
+__device__ __forceinline__ void ClusterArrive()
+{
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void ClusterWait()
+{
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void ClusterSync()
 {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    ClusterArrive();
+    ClusterWait();
 }
 // word of another CTA of the cluster at the place of `mine` in its shared memory
 __device__ __forceinline__ unsigned ClusterAddress(const void *mine, int rank)

@@ -165,12 +165,14 @@ struct TSelectParams {
     int *Status;
 };
 
-constexpr int SEL_THREADS = 512;
-constexpr int SEL_WARPS = SEL_THREADS / 32;
 constexpr int SEL_BINS = 2048;            // 11, 11 and 10 bits of the order
 constexpr int SEL_MAX_CLUSTER = 8;
 constexpr int SEL_SLOTS = 4096;           // slots of a CTA where there are CTAs enough
-constexpr int SEL_MAX_SLICE = 48 * 1024;  // slots whose orders fit shared memory
+constexpr int SEL_LIST = 2048;            // orders of a CTA that are counted from a list instead of from all
+constexpr int SEL_THREADS = 256;          // of a CTA; 1024 where there are too few CTAs
+constexpr int SEL_PER_SM = 4;
+constexpr int SEL_AHEAD = 2;              // steps of a warp whose loads are under way together
+constexpr int SEL_MAX_SLICE = 44 * 1024;  // slots whose orders fit shared memory
 
 // weights as unsigned integers of the same order; -0 counts as 0, NaN as the greatest; tokens that stay whatever their weight are above all
 constexpr unsigned SEL_PINNED = 0xffffffffu, SEL_NAN = 0xfffffffeu;
@@ -180,25 +182,45 @@ __device__ __forceinline__ unsigned WeightOrder(float w)
     return w != w ? SEL_NAN : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-// orders of slots slot .. slot + 3 (slot a multiple of 4); slots of pages outside the pool are the lightest
-__device__ __forceinline__ uint4 SlotOrders(const TSelectParams &p, const int *table, int head, int slot, int newest, bool *bad)
+// weights and positions of slots slot .. slot + 3 (slot a multiple of 4)
+struct TSlotWeights {
+    float4 W;
+    int4 Pos;
+    bool Ok; // the page is in the pool
+};
+__device__ __forceinline__ int SlotPage(const TSelectParams &p, const int *table, int slot)
+{
+    return table[slot >> p.C.PageShift];
+}
+__device__ __forceinline__ TSlotWeights LoadWeights(const TSelectParams &p, int page, int head, int slot)
 {
     const TPages &c = p.C;
-    const int page = table[slot >> c.PageShift];
-    if ((unsigned)page >= (unsigned)c.PageCount) {
-        *bad = true;
+    TSlotWeights r;
+    r.W = make_float4(0, 0, 0, 0);
+    r.Pos = make_int4(slot, slot + 1, slot + 2, slot + 3);
+    r.Ok = (unsigned)page < (unsigned)c.PageCount;
+    if (r.Ok) {
+        const size_t at = PlaneSlot(c, page, head) + (slot & ((1 << c.PageShift) - 1));
+        r.W = *reinterpret_cast<const float4 *>(c.Weight + at);
+        if (p.Recent > 0 && c.Pos) {
+            r.Pos = *reinterpret_cast<const int4 *>(c.Pos + at);
+        }
+    }
+    return r;
+}
+// their orders; slots of pages outside the pool are the lightest
+__device__ __forceinline__ uint4 SlotOrders(const TSelectParams &p, const TSlotWeights &x, int newest)
+{
+    if (!x.Ok) {
         return make_uint4(0, 0, 0, 0);
     }
-    const size_t at = PlaneSlot(c, page, head) + (slot & ((1 << c.PageShift) - 1));
-    const float4 w = *reinterpret_cast<const float4 *>(c.Weight + at);
-    uint4 o = make_uint4(WeightOrder(w.x), WeightOrder(w.y), WeightOrder(w.z), WeightOrder(w.w));
+    uint4 o = make_uint4(WeightOrder(x.W.x), WeightOrder(x.W.y), WeightOrder(x.W.z), WeightOrder(x.W.w));
     if (p.Recent > 0) {
-        const int4 pos = c.Pos ? *reinterpret_cast<const int4 *>(c.Pos + at) : make_int4(slot, slot + 1, slot + 2, slot + 3);
         const int old = newest - p.Recent;
-        o.x = pos.x > old ? SEL_PINNED : o.x;
-        o.y = pos.y > old ? SEL_PINNED : o.y;
-        o.z = pos.z > old ? SEL_PINNED : o.z;
-        o.w = pos.w > old ? SEL_PINNED : o.w;
+        o.x = x.Pos.x > old ? SEL_PINNED : o.x;
+        o.y = x.Pos.y > old ? SEL_PINNED : o.y;
+        o.z = x.Pos.z > old ? SEL_PINNED : o.z;
+        o.w = x.Pos.w > old ? SEL_PINNED : o.w;
     }
     return o;
 }
@@ -210,30 +232,91 @@ __device__ __forceinline__ uint4 ClusterLoad16(unsigned address)
     return r;
 }
 
+__device__ __forceinline__ void ClusterAdd(unsigned address, unsigned x)
+{
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(address), "r"(x) : "memory");
+}
+
+template <int WARPS>
 struct TSelectShared {
-    unsigned Hist[3][SEL_BINS];
-    int WarpSum[SEL_WARPS];
-    int Found[2];            // bin, and how many are still to be taken from it
-    int4 Total;              // of this CTA: ties, holes, movers
-    int4 WarpOf[SEL_WARPS];
+    alignas(16) unsigned Hist[3][SEL_BINS];
+    unsigned List[SEL_LIST];  // orders that agree with the first digit
+    int ListLen;
+    alignas(16) int Found[4]; // bin, how many are still to be taken from it, how many it has
+    int4 Total;               // of this CTA: ties, holes, movers
+    int4 WarpOf[WARPS];
 };
+
+// sum of the values of the warps before this one, and of all (values in shared memory)
+template <int WARPS>
+__device__ __forceinline__ int WarpsBefore(int mine, int warp, int lane, int *all)
+{
+    const int v = lane < WARPS ? mine : 0;
+    *all = __reduce_add_sync(0xffffffffu, v);
+    return __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+}
+
+// The largest bin at which the sum of the counts from the last bin down reaches `take`: found[0]; how many are to be taken from it: found[1];
+// its count: found[2].  One warp: lane l has bins SEL_BINS - 64 (l + 1) .. + 63, then the lane that has the bin looks for it in its own.
+__device__ __forceinline__ void FindBin(const unsigned *hist, int lane, int take, int *found)
+{
+    constexpr int PER = SEL_BINS / 32;
+    const int first = SEL_BINS - PER * (lane + 1);
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) {
+        const uint4 h = *reinterpret_cast<const uint4 *>(hist + first + 4 * ((i + lane) % (PER / 4))); // turned by the lane: no two in a bank
+        mine += (int)(h.x + h.y + h.z + h.w);
+    }
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        sum += lane >= o ? v : 0;
+    }
+    // the lane that has the bin, then its 64 bins two to a lane
+    const unsigned reach = __ballot_sync(0xffffffffu, sum >= take);
+    const int who = reach ? __ffs(reach) - 1 : 31;
+    const int above = __shfl_sync(0xffffffffu, sum - mine, who), base = SEL_BINS - PER * (who + 1);
+    const uint2 two = *reinterpret_cast<const uint2 *>(hist + base + PER - 2 * (lane + 1)); // two.y is the larger bin
+    const int pair = (int)(two.x + two.y);
+    sum = pair;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        sum += lane >= o ? v : 0;
+    }
+    const int before = above + sum - pair;
+    if (before < take && above + sum >= take) {
+        const bool larger = before + (int)two.y >= take;
+        found[0] = base + PER - 2 * (lane + 1) + (larger ? 1 : 0);
+        found[1] = take - before - (larger ? 0 : (int)two.y);
+        found[2] = larger ? two.y : two.x;
+    }
+}
 
 // One cluster of CTAs per (sequence, key head); CTA `rank` has the slots [rank * slice, (rank + 1) * slice), each warp a contiguous run of
 // them, four to a lane.  The keep-th largest order is found in three digits: counts of the digit among the orders that agree in the digits
-// before (shared memory, the CTAs' counts added through distributed shared memory), then the sum from the top.  Ranks in slot order are
-// ballots on top of the sums of the warps and CTAs before.  CACHED: the orders stay in shared memory after they are read once.
-template <bool CACHED>
-__global__ void __launch_bounds__(SEL_THREADS) PagedSelectKernel(const TSelectParams p)
+// before (shared memory; a cluster's CTAs add theirs to the first one's, which finds the digit), then the sum from the top.  The orders that agree with
+// the first digit are few: they go into a list, which the other digits are counted from.  Ranks in slot order are ballots on top of the
+// sums of the warps and CTAs before.  CACHED: the orders stay in shared memory after they are read once.
+template <int THREADS, bool CACHED>
+__global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM : 1) PagedSelectKernel(const TSelectParams p)
 {
+    constexpr int WARPS = THREADS / 32;
     extern __shared__ uint4 cached[];
-    __shared__ __align__(16) TSelectShared sh;
+    __shared__ __align__(16) TSelectShared<WARPS> sh;
     const int head = blockIdx.x / p.Cluster, rank = blockIdx.x % p.Cluster, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const unsigned below = (1u << lane) - 1;
     const TPages &c = p.C;
-    for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) {
-        sh.Hist[0][i] = 0;
+    PdlTrigger();
+    for (int i = tid; i < 3 * SEL_BINS / 4; i += THREADS) {
+        reinterpret_cast<uint4 *>(sh.Hist)[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (tid == 0) {
+        sh.ListLen = 0;
     }
     PdlWait();
-    PdlTrigger();
     const int len = p.CtxLens[seq];
     const size_t unit = (size_t)seq * c.KvHeads + head;
     int2 *moves = p.Moves + unit * p.MoveCap;
@@ -251,7 +334,7 @@ __global__ void __launch_bounds__(SEL_THREADS) PagedSelectKernel(const TSelectPa
         }
     }
     if (none) { // the same in all CTAs of the cluster
-        for (int i = rank * SEL_THREADS + tid; i < p.MoveCap; i += p.Cluster * SEL_THREADS) {
+        for (int i = rank * THREADS + tid; i < p.MoveCap; i += p.Cluster * THREADS) {
             moves[i] = make_int2(-1, -1);
         }
         return;
@@ -259,107 +342,155 @@ __global__ void __launch_bounds__(SEL_THREADS) PagedSelectKernel(const TSelectPa
     const int *table = c.Table.Row(seq);
     const int newest = (p.Tokens ? p.Tokens[seq] : len) - 1;
     // slots of a CTA and of a warp: equal parts of what the sequence has, in whole steps of 128
-    const int warps = p.Cluster * SEL_WARPS;
+    const int warps = p.Cluster * WARPS;
     const int per = ((len + warps - 1) / warps + 127) & ~127;
-    const int slice = per * SEL_WARPS;
+    const int slice = per * WARPS;
     const int beg = min(rank * slice + warp * per, len), end = min(beg + per, len);
     bool bad = false;
-    auto orders = [&](int s) { return CACHED ? cached[(s - rank * slice) >> 2] : SlotOrders(p, table, head, s, newest, &bad); };
-    auto count = [&](unsigned *hist, unsigned bin, bool in) {
-        // equal bins of a whole warp (weights that are all zero) are one addition
-        const unsigned first = __shfl_sync(0xffffffffu, bin, 0);
-        if (__all_sync(0xffffffffu, in && bin == first)) {
+    auto orders = [&](int s) {
+        if (CACHED) {
+            return cached[(s - rank * slice) >> 2];
+        }
+        return SlotOrders(p, LoadWeights(p, SlotPage(p, table, s), head, s), newest);
+    };
+    // one more in the bin of each order that is in: (order >> shift) & low; equal bins of a whole step (weights that are all zero) are one addition
+    auto count = [&](unsigned *hist, const uint4 &o, int shift, unsigned low, unsigned in) {
+        const unsigned x = o.x >> shift & low, y = o.y >> shift & low, z = o.z >> shift & low, w = o.w >> shift & low;
+        const unsigned first = __shfl_sync(0xffffffffu, x, 0);
+        if (__all_sync(0xffffffffu, in == 15 && x == first && y == first && z == first && w == first)) {
             if (lane == 0) {
-                atomicAdd(hist + bin, 32);
+                atomicAdd(hist + first, 128);
             }
-        } else if (in) {
-            atomicAdd(hist + bin, 1);
+        } else {
+            if (in & 1) {
+                atomicAdd(hist + x, 1);
+            }
+            if (in & 2) {
+                atomicAdd(hist + y, 1);
+            }
+            if (in & 4) {
+                atomicAdd(hist + z, 1);
+            }
+            if (in & 8) {
+                atomicAdd(hist + w, 1);
+            }
         }
     };
+    // of four slots from s on, the ones below `limit`
+    auto until = [](int s, int limit) { return (1u << max(0, min(4, limit - s))) - 1; };
+    // of four orders, the ones that agree with the digits found so far
+    auto agree = [](const uint4 &o, unsigned mask, unsigned cut) {
+        return (unsigned)((o.x & mask) == cut) | (unsigned)((o.y & mask) == cut) << 1 | (unsigned)((o.z & mask) == cut) << 2 | (unsigned)((o.w & mask) == cut) << 3;
+    };
     __syncthreads(); // the counts are zero
-#pragma unroll 2
-    for (int s0 = beg; s0 < end; s0 += 128) {
-        const int s = s0 + 4 * lane;
-        uint4 o = make_uint4(0, 0, 0, 0);
-        if (s < end) {
-            o = SlotOrders(p, table, head, s, newest, &bad);
-            if (CACHED) {
-                cached[(s - rank * slice) >> 2] = o;
-            }
+    if (p.Cluster > 1) {
+        ClusterArrive();
+    }
+    for (int s0 = beg; s0 < end; s0 += 128 * SEL_AHEAD) {
+        int page[SEL_AHEAD];
+        TSlotWeights x[SEL_AHEAD];
+#pragma unroll
+        for (int j = 0; j < SEL_AHEAD; ++j) {
+            const int s = s0 + 128 * j + 4 * lane;
+            page[j] = s < end ? SlotPage(p, table, s) : -1;
         }
-        count(sh.Hist[0], o.x >> 21, s < end);
-        count(sh.Hist[0], o.y >> 21, s + 1 < end);
-        count(sh.Hist[0], o.z >> 21, s + 2 < end);
-        count(sh.Hist[0], o.w >> 21, s + 3 < end);
+#pragma unroll
+        for (int j = 0; j < SEL_AHEAD; ++j) {
+            x[j] = LoadWeights(p, page[j], head, s0 + 128 * j + 4 * lane);
+        }
+#pragma unroll
+        for (int j = 0; j < SEL_AHEAD; ++j) {
+            const int s = s0 + 128 * j + 4 * lane;
+            if (s0 + 128 * j >= end) {
+                break;
+            }
+            const uint4 o = SlotOrders(p, x[j], newest);
+            if (s < end) {
+                bad |= !x[j].Ok;
+                if (CACHED) {
+                    cached[(s - rank * slice) >> 2] = o;
+                }
+            }
+            count(sh.Hist[0], o, 21, 2047, until(s, end));
+        }
     }
     unsigned cut = 0;     // the digits found so far
     int take = p.Keep;    // how many of the orders that agree with them stay
+    int equal = 0;        // how many agree
 #pragma unroll
     for (int digit = 0; digit < 3; ++digit) {
         constexpr int SHIFT[3] = {21, 10, 0};
-        const int bits = digit == 2 ? 10 : 11;
-        if (digit > 0) {
-            const unsigned mask = digit == 1 ? 0xffe00000u : 0xfffffc00u;
+        constexpr unsigned low = 1023;
+        if (digit == 1) {
             for (int s0 = beg; s0 < end; s0 += 128) {
                 const int s = s0 + 4 * lane;
-                const uint4 o = s < end ? orders(s) : make_uint4(0, 0, 0, 0);
-                const unsigned low = (1u << bits) - 1;
-                const bool x = s < end && (o.x & mask) == cut, y = s + 1 < end && (o.y & mask) == cut;
-                const bool z = s + 2 < end && (o.z & mask) == cut, w = s + 3 < end && (o.w & mask) == cut;
-                if (__any_sync(0xffffffffu, x | y | z | w)) {
-                    count(sh.Hist[digit], o.x >> SHIFT[digit] & low, x);
-                    count(sh.Hist[digit], o.y >> SHIFT[digit] & low, y);
-                    count(sh.Hist[digit], o.z >> SHIFT[digit] & low, z);
-                    count(sh.Hist[digit], o.w >> SHIFT[digit] & low, w);
+                const uint4 o4 = s < end ? orders(s) : make_uint4(0, 0, 0, 0);
+                const unsigned in = until(s, end) & agree(o4, 0xffe00000u, cut);
+                if (__any_sync(0xffffffffu, in)) {
+                    const unsigned o[4] = {o4.x, o4.y, o4.z, o4.w};
+                    int at = in ? atomicAdd(&sh.ListLen, __popc(in)) : 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (in >> i & 1) {
+                            if (at < SEL_LIST) {
+                                sh.List[at] = o[i];
+                            }
+                            ++at;
+                        }
+                    }
+                    count(sh.Hist[1], o4, 10, 2047, in);
+                }
+            }
+        } else if (digit == 2) {
+            if (sh.ListLen <= SEL_LIST) {
+                for (int i = tid; i < sh.ListLen; i += THREADS) {
+                    const unsigned o = sh.List[i];
+                    if ((o & 0xfffffc00u) == cut) {
+                        atomicAdd(&sh.Hist[2][o & 1023], 1);
+                    }
+                }
+            } else {
+                for (int s0 = beg; s0 < end; s0 += 128) {
+                    const int s = s0 + 4 * lane;
+                    const uint4 o = s < end ? orders(s) : make_uint4(0, 0, 0, 0);
+                    count(sh.Hist[2], o, 0, low, until(s, end) & agree(o, 0xfffffc00u, cut));
                 }
             }
         }
+        __syncthreads();
+        if (p.Cluster > 1) {
+            // the first CTA's counts become those of the cluster
+            if (digit == 0) {
+                ClusterWait(); // they were zero
+            }
+            if (rank > 0) {
+                for (int i = tid; i < SEL_BINS; i += THREADS) {
+                    const unsigned n = sh.Hist[digit][i];
+                    if (n) {
+                        ClusterAdd(ClusterAddress(&sh.Hist[digit][i], 0), n);
+                    }
+                }
+            }
+            ClusterSync();
+        }
+        if (rank == 0 && warp == 0) {
+            FindBin(sh.Hist[digit], lane, take, sh.Found);
+        }
         if (p.Cluster > 1) {
             ClusterSync();
+            const uint4 found = ClusterLoad16(ClusterAddress(sh.Found, 0));
+            cut |= found.x << SHIFT[digit];
+            take = (int)found.y;
+            equal = (int)found.z;
         } else {
             __syncthreads();
+            cut |= (unsigned)sh.Found[0] << SHIFT[digit];
+            take = sh.Found[1];
+            equal = sh.Found[2];
         }
-        // thread t has bins [top - 4 t - 3, top - 4 t]: sums run from the largest bin down
-        const int first = (1 << 11) - 4 - 4 * tid; // digits of 10 bits use the lower half, the rest is zero
-        uint4 h = *reinterpret_cast<const uint4 *>(&sh.Hist[digit][first]);
-        for (int r = 1; r < p.Cluster; ++r) {
-            const uint4 o = ClusterLoad16(ClusterAddress(&sh.Hist[digit][first], (rank + r) % p.Cluster));
-            h.x += o.x;
-            h.y += o.y;
-            h.z += o.z;
-            h.w += o.w;
-        }
-        const int mine = (int)(h.x + h.y + h.z + h.w);
-        int sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            sum += lane >= o ? v : 0;
-        }
-        if (lane == 31) {
-            sh.WarpSum[warp] = sum;
-        }
-        __syncthreads();
-        for (int w = 0; w < warp; ++w) {
-            sum += sh.WarpSum[w];
-        }
-        int above = sum - mine; // orders in larger bins
-        if (above < take && sum >= take) {
-            const unsigned b[4] = {h.w, h.z, h.y, h.x};
-            int i = 0;
-            while (above + (int)b[i] < take) {
-                above += b[i++];
-            }
-            sh.Found[0] = first + 3 - i;
-            sh.Found[1] = take - above;
-            sh.Total.w = b[i]; // how many agree
-        }
-        __syncthreads();
-        cut |= (unsigned)sh.Found[0] << SHIFT[digit];
-        take = sh.Found[1];
     }
     // `take` of the orders equal to cut stay, the first ones in slot order; mostly that is all of them
-    const bool allTies = sh.Total.w == take;
+    const bool allTies = equal == take;
     int ties = take;
     if (!allTies) {
         int n = 0;
@@ -375,11 +506,8 @@ __global__ void __launch_bounds__(SEL_THREADS) PagedSelectKernel(const TSelectPa
             sh.WarpOf[warp].x = n;
         }
         __syncthreads();
-        int before = 0, total = 0;
-        for (int w = 0; w < SEL_WARPS; ++w) {
-            before += w < warp ? sh.WarpOf[w].x : 0;
-            total += sh.WarpOf[w].x;
-        }
+        int total;
+        int before = WarpsBefore<WARPS>(lane < WARPS ? sh.WarpOf[lane].x : 0, warp, lane, &total);
         if (p.Cluster > 1) {
             if (tid == 0) {
                 sh.Total.x = total;
@@ -391,98 +519,86 @@ __global__ void __launch_bounds__(SEL_THREADS) PagedSelectKernel(const TSelectPa
         }
         ties -= before; // left for this warp's slots
     }
-    // two sweeps: count, then write
-    int hole = 0, mover = 0, moved = 0;
-#pragma unroll
-    for (int sweep = 0; sweep < 2; ++sweep) {
-        int left = ties;
-        for (int s0 = beg; s0 < end; s0 += 128) {
-            const int s = s0 + 4 * lane;
-            const uint4 o4 = s < end ? orders(s) : make_uint4(0, 0, 0, 0);
-            const unsigned o[4] = {o4.x, o4.y, o4.z, o4.w};
-            const unsigned below = (1u << lane) - 1;
-            bool keep[4];
-            if (allTies) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    keep[i] = s + i < end && o[i] >= cut;
-                }
-            } else {
-                unsigned tie[4];
-                int before = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    tie[i] = __ballot_sync(0xffffffffu, s + i < end && o[i] == cut);
-                    before += __popc(tie[i] & below);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool mine = tie[i] >> lane & 1;
-                    keep[i] = s + i < end && (o[i] > cut || (mine && before < left));
-                    before += mine;
-                }
-                left -= __popc(tie[0]) + __popc(tie[1]) + __popc(tie[2]) + __popc(tie[3]);
-            }
-            int hb = 0, mb = 0, hn = 0, mn = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned h = __ballot_sync(0xffffffffu, s + i < end && !keep[i] && s + i < p.Keep);
-                const unsigned m = __ballot_sync(0xffffffffu, keep[i] && s + i >= p.Keep);
-                hb += __popc(h & below);
-                mb += __popc(m & below);
-                hn += __popc(h);
-                mn += __popc(m);
-            }
-            if (sweep) {
-                int hr = hole + hb, mr = mover + mb;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (s + i < end && !keep[i] && s + i < p.Keep && hr < p.MoveCap) {
-                        moves[hr++].x = s + i;
-                    }
-                    if (keep[i] && s + i >= p.Keep && mr < p.MoveCap) {
-                        moves[mr++].y = s + i;
-                    }
-                }
-            }
-            hole += hn;
-            mover += mn;
+    // one slot per lane from here on
+    auto order = [&](int s) {
+        if (CACHED) {
+            return reinterpret_cast<const unsigned *>(cached)[s - rank * slice];
         }
-        if (!sweep) {
-            if (lane == 0) {
-                sh.WarpOf[warp] = make_int4(0, hole, mover, 0);
-            }
-            __syncthreads();
-            int4 total = make_int4(0, 0, 0, 0);
-            hole = mover = 0;
-            for (int w = 0; w < SEL_WARPS; ++w) {
-                const int4 x = sh.WarpOf[w];
-                hole += w < warp ? x.y : 0;
-                mover += w < warp ? x.z : 0;
-                total.y += x.y;
-                total.z += x.z;
-            }
-            moved = total.z;
-            if (p.Cluster > 1) {
-                ClusterSync(); // the ties of Total have been read
-                if (tid == 0) {
-                    sh.Total = total;
-                }
-                ClusterSync();
-                for (int r = 0; r < p.Cluster; ++r) {
-                    const uint4 x = ClusterLoad16(ClusterAddress(&sh.Total, r));
-                    hole += r < rank ? (int)x.y : 0;
-                    mover += r < rank ? (int)x.z : 0;
-                    moved += r != rank ? (int)x.z : 0;
-                }
-            }
-            for (int i = moved + rank * SEL_THREADS + tid; i < p.MoveCap; i += p.Cluster * SEL_THREADS) {
-                moves[i] = make_int2(-1, -1);
-            }
-            if (tid == 0 && rank == 0) {
-                p.Counts[unit] = min(moved, p.MoveCap);
-            }
+        const uint4 o = orders(s & ~3);
+        return s & 2 ? (s & 1 ? o.w : o.z) : (s & 1 ? o.y : o.x);
+    };
+    // whether slot s stays; `left`: of the ties
+    auto kept = [&](int s, int &left) {
+        const unsigned o = s < end ? order(s) : 0;
+        bool k = s < end && o >= cut;
+        if (!allTies) {
+            const unsigned tie = __ballot_sync(0xffffffffu, k && o == cut);
+            k = k && (o > cut || __popc(tie & below) < left);
+            left -= __popc(tie);
         }
+        return k;
+    };
+    // slots that leave a hole in front of the budget, or that are moved from behind it
+    int hole = 0, mover = 0, left = ties;
+    for (int s0 = beg; s0 < end; s0 += 32) {
+        const int s = s0 + lane;
+        const bool k = kept(s, left);
+        hole += s < p.Keep && s < end && !k;
+        mover += s >= p.Keep && k;
+    }
+    hole = __reduce_add_sync(0xffffffffu, hole);
+    mover = __reduce_add_sync(0xffffffffu, mover);
+    __syncthreads(); // WarpOf has been read
+    if (lane == 0) {
+        sh.WarpOf[warp] = make_int4(0, hole, mover, 0);
+    }
+    __syncthreads();
+    const int4 of = lane < WARPS ? sh.WarpOf[lane] : make_int4(0, 0, 0, 0);
+    int4 total = make_int4(0, 0, 0, 0);
+    hole = WarpsBefore<WARPS>(of.y, warp, lane, &total.y);
+    mover = WarpsBefore<WARPS>(of.z, warp, lane, &total.z);
+    int moved = total.z;
+    if (p.Cluster > 1) {
+        ClusterSync(); // the ties of Total have been read
+        if (tid == 0) {
+            sh.Total = total;
+        }
+        ClusterSync();
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (lane < p.Cluster) {
+            x = ClusterLoad16(ClusterAddress(&sh.Total, lane));
+        }
+        moved = __reduce_add_sync(0xffffffffu, (int)x.z);
+        hole += __reduce_add_sync(0xffffffffu, lane < rank ? (int)x.y : 0);
+        mover += __reduce_add_sync(0xffffffffu, lane < rank ? (int)x.z : 0);
+    }
+    // (as many of each as there is room for: at most min(keep, len - keep))
+    left = ties;
+    for (int s0 = beg; s0 < end; s0 += 32) {
+        const int s = s0 + lane;
+        const bool k = kept(s, left);
+        if (s0 < p.Keep) {
+            const bool is = s < p.Keep && s < end && !k;
+            const unsigned all = __ballot_sync(0xffffffffu, is);
+            if (is) {
+                moves[hole + __popc(all & below)].x = s;
+            }
+            hole += __popc(all);
+        }
+        if (s0 + 32 > p.Keep) {
+            const bool is = s >= p.Keep && k;
+            const unsigned all = __ballot_sync(0xffffffffu, is);
+            if (is) {
+                moves[mover + __popc(all & below)].y = s;
+            }
+            mover += __popc(all);
+        }
+    }
+    for (int i = moved + rank * THREADS + tid; i < p.MoveCap; i += p.Cluster * THREADS) {
+        moves[i] = make_int2(-1, -1);
+    }
+    if (tid == 0 && rank == 0) {
+        p.Counts[unit] = moved;
     }
     if (bad && p.Status) {
         atomicOr(p.Status, kDevBadSpan);
@@ -658,24 +774,27 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_evict_select(con
     if (rc != TSA_OK) {
         return rc;
     }
-    // CTAs of SEL_SLOTS slots while all of them are resident at once (four to an SM)
+    // CTAs of SEL_SLOTS slots while all of them are resident at once (four to an SM); where even then a CTA has twice as many, of twice the
+    // threads
     p.Cluster = 1;
     while (p.Cluster < SEL_MAX_CLUSTER && longest > SEL_SLOTS * p.Cluster && 2ll * p.Cluster * kv->kv_heads * nSeq <= 4ll * sms) {
         p.Cluster *= 2;
     }
-    const int warps = p.Cluster * SEL_WARPS;
-    const int slice = ((longest + warps - 1) / warps + 127) / 128 * 128 * SEL_WARPS;
+    const bool many = longest > 2 * SEL_SLOTS * p.Cluster;
+    const int threads = many ? 1024 : SEL_THREADS, warps = p.Cluster * threads / 32;
+    const int slice = ((longest + warps - 1) / warps + 127) / 128 * 128 * (threads / 32);
     const bool cached = slice <= SEL_MAX_SLICE;
-    const void *kern = cached ? (const void *)PagedSelectKernel<true> : (const void *)PagedSelectKernel<false>;
+    const void *kern = many ? (cached ? (const void *)PagedSelectKernel<1024, true> : (const void *)PagedSelectKernel<1024, false>)
+                            : (const void *)PagedSelectKernel<SEL_THREADS, true>;
     const size_t smem = cached ? (size_t)slice * sizeof(unsigned) : 0;
-    if (smem > 16 * 1024) { // beyond 48 KB with the counts
-        rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_SLICE * sizeof(unsigned)), "cudaFuncSetAttribute");
+    if (smem > 8 * 1024) { // beyond 48 KB with the counts
+        rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
         if (rc != TSA_OK) {
             return rc;
         }
     }
     void *args[] = {&p};
-    return CheckCuda(LaunchPdl(kern, dim3(kv->kv_heads * p.Cluster, nSeq), dim3(SEL_THREADS), smem, (cudaStream_t)stream, args, p.Cluster),
+    return CheckCuda(LaunchPdl(kern, dim3(kv->kv_heads * p.Cluster, nSeq), dim3(threads), smem, (cudaStream_t)stream, args, p.Cluster),
         "tsa_paged_evict_select launch");
 }
 
