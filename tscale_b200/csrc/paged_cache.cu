@@ -4,6 +4,7 @@
 // Layout: a page holds page_size tokens of all key heads, head by head, so that what one head reads of a page is one contiguous block of
 // page_size * D bytes of K and as many of V.  All planes (scales, positions, weights) have the same [page][head][slot] order.
 #include "paged.cuh"
+#include <type_traits>
 
 namespace tsa {
 
@@ -56,7 +57,7 @@ struct TAppendParams {
     int *Status;
 };
 
-constexpr int APP_WARPS = 4;
+constexpr int APP_WARPS = 8;
 
 // the sequence whose rows [starts[s], starts[s + 1]) hold `row`: the last s with starts[s] <= row, -1 if row is in front of all or behind the
 // last.  A warp narrows the range by 33 per step (sequences without rows have equal starts and are stepped over).
@@ -77,65 +78,97 @@ __device__ __forceinline__ int FindSeq(const int *starts, int nSeq, int row, int
     return lo;
 }
 
-// One warp per row: it finds the row's sequence, slot and page, and copies the row's heads 16 bytes a lane.
+// One warp per row: it finds the row's sequence, slot and page while the row's first 64 pieces of 16 bytes of K and V are on their way, and
+// stores the heads' pieces.  The warps of a CTA have neighbouring rows, which are neighbours in their page, too: scales, positions and
+// weights are stored by all of them, a sector of eight rows at a time.
 template <int D, bool SCALE_F16>
 __global__ void __launch_bounds__(APP_WARPS * 32) PagedAppendKernel(const TAppendParams p)
 {
-    constexpr int LPH = D / 16;
-    const int lane = threadIdx.x & 31;
-    const int row = blockIdx.x * APP_WARPS + (threadIdx.x >> 5);
+    constexpr int LPH = D / 16, AHEAD = 4;
+    constexpr size_t NOWHERE = ~(size_t)0;
+    __shared__ size_t firstOf[APP_WARPS]; // where the rows' tokens are in the planes of head 0
+    __shared__ int posOf[APP_WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row0 = blockIdx.x * APP_WARPS, row = row0 + warp;
     PdlTrigger();
     PdlWait();
-    if (row >= p.Rows) {
-        return;
-    }
-    int seq = row, back = 1;
-    if (p.RowStarts) {
-        seq = FindSeq(p.RowStarts, p.NSeq, row, lane);
-        if (seq < 0) {
-            return;
-        }
-        back = p.RowStarts[seq + 1] - row;
-    }
     const TPages &c = p.C;
-    const int slot = p.CtxLens[seq] - back;
-    const int col = slot >> c.PageShift;
-    int page = -1;
-    if (slot >= 0 && col < c.TableCols) {
-        page = c.Table.Row(seq)[col];
-    }
-    if (page < 0 || page >= c.PageCount) {
-        if (lane == 0 && p.Status) {
-            atomicOr(p.Status, kDevBadSpan); // no such place: nothing is stored
-        }
-        return;
-    }
-    const int inPage = slot & ((1 << c.PageShift) - 1);
-    const size_t first = PlaneSlot(c, page, 0) + inPage; // of head 0; the next head's is a page of slots further
-    const int pieces = c.KvHeads * LPH;
-    const int4 *ks = reinterpret_cast<const int4 *>(p.KNew.Row(row)), *vs = reinterpret_cast<const int4 *>(p.VNew.Row(row));
-    for (int i = lane; i < pieces; i += 128) {
-        int4 a[4], b[4];
+    const int pieces = row < p.Rows ? c.KvHeads * LPH : 0;
+    const int4 *ks = nullptr, *vs = nullptr;
+    int4 a[AHEAD], b[AHEAD];
+    auto load = [&](int i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < AHEAD; ++j) {
             if (i + j * 32 < pieces) {
                 a[j] = __ldg(ks + i + j * 32);
                 b[j] = __ldg(vs + i + j * 32);
             }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int x = i + j * 32;
-            if (x < pieces) {
-                const size_t at = (first + ((size_t)(x / LPH) << c.PageShift)) * LPH + x % LPH;
-                reinterpret_cast<int4 *>(c.K)[at] = a[j];
-                reinterpret_cast<int4 *>(c.V)[at] = b[j];
+    };
+    // the scales that this thread will store: of head h0 and row r of the CTA
+    const int r = tid % APP_WARPS, h0 = tid / APP_WARPS;
+    float sk = 0, sv = 0;
+    if (h0 < c.KvHeads && row0 + r < p.Rows) {
+        sk = p.KScaleNew.Row(h0)[row0 + r];
+        sv = p.VScaleNew.Row(h0)[row0 + r];
+    }
+    size_t first = NOWHERE;
+    if (row < p.Rows) {
+        ks = reinterpret_cast<const int4 *>(p.KNew.Row(row));
+        vs = reinterpret_cast<const int4 *>(p.VNew.Row(row));
+        load(lane);
+        int seq = row, back = 1;
+        if (p.RowStarts) {
+            seq = FindSeq(p.RowStarts, p.NSeq, row, lane);
+            back = seq < 0 ? 0 : p.RowStarts[seq + 1] - row;
+        }
+        if (seq >= 0) {
+            const int len = p.CtxLens[seq], slot = len - back, col = slot >> c.PageShift;
+            int page = -1;
+            if (slot >= 0 && col < c.TableCols) {
+                page = c.Table.Row(seq)[col];
+            }
+            if ((unsigned)page < (unsigned)c.PageCount) {
+                first = PlaneSlot(c, page, 0) + (slot & ((1 << c.PageShift) - 1)); // the next head's is a page of slots further
+                if (lane == 0) {
+                    posOf[warp] = (p.Tokens ? p.Tokens[seq] : len) - back;
+                }
+            } else if (lane == 0 && p.Status) {
+                atomicOr(p.Status, kDevBadSpan); // no such place: nothing is stored
             }
         }
     }
-    for (int h = lane; h < c.KvHeads; h += 32) {
-        const size_t at = first + ((size_t)h << c.PageShift);
-        const float sk = p.KScaleNew.Row(h)[row], sv = p.VScaleNew.Row(h)[row];
+    if (lane == 0) {
+        firstOf[warp] = first;
+    }
+    if (first != NOWHERE) {
+        for (int i = lane;;) {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int x = i + j * 32;
+                if (x < pieces) {
+                    const size_t at = (first + ((size_t)(x / LPH) << c.PageShift)) * LPH + x % LPH;
+                    reinterpret_cast<int4 *>(c.K)[at] = a[j];
+                    reinterpret_cast<int4 *>(c.V)[at] = b[j];
+                }
+            }
+            i += 32 * AHEAD;
+            if (i - lane >= pieces) {
+                break;
+            }
+            load(i);
+        }
+    }
+    __syncthreads();
+    if (firstOf[r] == NOWHERE) {
+        return;
+    }
+    for (int h = h0; h < c.KvHeads; h += 32) {
+        const size_t at = firstOf[r] + ((size_t)h << c.PageShift);
+        if (h > h0) {
+            sk = p.KScaleNew.Row(h)[row0 + r];
+            sv = p.VScaleNew.Row(h)[row0 + r];
+        }
         if (SCALE_F16) {
             reinterpret_cast<__half *>(c.KScale)[at] = __float2half_rn(sk);
             reinterpret_cast<__half *>(c.VScale)[at] = __float2half_rn(sv);
@@ -144,7 +177,7 @@ __global__ void __launch_bounds__(APP_WARPS * 32) PagedAppendKernel(const TAppen
             reinterpret_cast<float *>(c.VScale)[at] = sv;
         }
         if (c.Pos) {
-            c.Pos[at] = (p.Tokens ? p.Tokens[seq] : p.CtxLens[seq]) - back;
+            c.Pos[at] = posOf[r];
         }
         if (c.Weight) {
             c.Weight[at] = 0.0f;
@@ -620,10 +653,13 @@ struct TMoveParams {
 constexpr int MOV_WARPS = 4;
 
 // A warp takes 32 moves: each lane looks up the pages of one and carries its scales, position and weight; then 2 D / 16 lanes at a time
-// carry a row of K and V.  Sources and destinations of a head are different slots (sources lie behind the budget), so no order is needed.
+// carry a row of K and V, MOV_AHEAD rows of a lane on their way together.  Sources and destinations of a head are different slots (sources
+// lie behind the budget), so no order is needed.
+constexpr int MOV_AHEAD = 8;
 template <int D, int SCALE_BYTES>
 __global__ void __launch_bounds__(MOV_WARPS * 32) PagedMoveKernel(const TMoveParams p)
 {
+    typedef typename std::conditional<SCALE_BYTES == 2, uint16_t, uint32_t>::type TScale;
     constexpr int LPM = 2 * D / 16, PER = 32 / LPM; // lanes per move, moves per step
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int head = blockIdx.y, seq = blockIdx.z;
@@ -631,12 +667,12 @@ __global__ void __launch_bounds__(MOV_WARPS * 32) PagedMoveKernel(const TMovePar
     PdlWait();
     const TPages &c = p.C;
     const size_t unit = (size_t)seq * c.KvHeads + head;
-    const int count = min(p.Counts[unit], p.MoveCap);
     const int base = (blockIdx.x * MOV_WARPS + warp) * 32;
+    const int2 *moves = p.Moves + unit * p.MoveCap;
+    const int count = min(p.Counts[unit], p.MoveCap);
     if (base >= count) {
         return;
     }
-    const int2 *moves = p.Moves + unit * p.MoveCap;
     const int *table = c.Table.Row(seq);
     const int mask = (1 << c.PageShift) - 1;
     bool ok = base + lane < count;
@@ -647,7 +683,7 @@ __global__ void __launch_bounds__(MOV_WARPS * 32) PagedMoveKernel(const TMovePar
         ok = m.x >= 0 && m.y >= 0 && m.x < room && m.y < room;
         if (ok) {
             const int pt = table[m.x >> c.PageShift], pf = table[m.y >> c.PageShift];
-            ok = pt >= 0 && pt < c.PageCount && pf >= 0 && pf < c.PageCount;
+            ok = (unsigned)pt < (unsigned)c.PageCount && (unsigned)pf < (unsigned)c.PageCount;
             if (ok) {
                 to = PlaneSlot(c, pt, head) + (m.x & mask);
                 of = PlaneSlot(c, pf, head) + (m.y & mask);
@@ -657,34 +693,47 @@ __global__ void __launch_bounds__(MOV_WARPS * 32) PagedMoveKernel(const TMovePar
             atomicOr(p.Status, kDevBadSpan);
         }
     }
-    const int n = min(32, count - base);
     const unsigned okMask = __ballot_sync(0xffffffffu, ok);
+    TScale sk = 0, sv = 0;
+    int pos = 0;
+    float weight = 0;
+    if (ok) {
+        sk = reinterpret_cast<const TScale *>(c.KScale)[of];
+        sv = reinterpret_cast<const TScale *>(c.VScale)[of];
+        pos = c.Pos ? c.Pos[of] : 0;
+        weight = c.Weight ? c.Weight[of] : 0.0f;
+    }
     const int sub = lane % LPM;
-    const uint8_t *pool = sub < D / 16 ? c.K : c.V;
+    int4 *const pool = reinterpret_cast<int4 *>(sub < D / 16 ? c.K : c.V);
     const int piece = sub % (D / 16);
-#pragma unroll 4
-    for (int i = 0; i < 32; i += PER) {
-        const int m = i + lane / LPM;
-        const size_t t = __shfl_sync(0xffffffffu, to, m), f = __shfl_sync(0xffffffffu, of, m);
-        if (m < n && (okMask >> m & 1)) {
-            reinterpret_cast<int4 *>((uint8_t *)pool)[t * (D / 16) + piece] = reinterpret_cast<const int4 *>(pool)[f * (D / 16) + piece];
+#pragma unroll 1
+    for (int i = 0; i < 32 && okMask >> i; i += PER * MOV_AHEAD) {
+        int4 x[MOV_AHEAD];
+#pragma unroll
+        for (int j = 0; j < MOV_AHEAD; ++j) {
+            const int m = i + j * PER + lane / LPM;
+            const size_t f = __shfl_sync(0xffffffffu, of, m & 31);
+            if (okMask >> (m & 31) & 1) {
+                x[j] = pool[f * (D / 16) + piece];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < MOV_AHEAD; ++j) {
+            const int m = i + j * PER + lane / LPM;
+            const size_t t = __shfl_sync(0xffffffffu, to, m & 31);
+            if (okMask >> (m & 31) & 1) {
+                pool[t * (D / 16) + piece] = x[j];
+            }
         }
     }
     if (ok) {
-        if (SCALE_BYTES == 2) {
-            const uint16_t a = reinterpret_cast<const uint16_t *>(c.KScale)[of], b = reinterpret_cast<const uint16_t *>(c.VScale)[of];
-            reinterpret_cast<uint16_t *>(c.KScale)[to] = a;
-            reinterpret_cast<uint16_t *>(c.VScale)[to] = b;
-        } else {
-            const uint32_t a = reinterpret_cast<const uint32_t *>(c.KScale)[of], b = reinterpret_cast<const uint32_t *>(c.VScale)[of];
-            reinterpret_cast<uint32_t *>(c.KScale)[to] = a;
-            reinterpret_cast<uint32_t *>(c.VScale)[to] = b;
-        }
+        reinterpret_cast<TScale *>(c.KScale)[to] = sk;
+        reinterpret_cast<TScale *>(c.VScale)[to] = sv;
         if (c.Pos) {
-            c.Pos[to] = c.Pos[of];
+            c.Pos[to] = pos;
         }
         if (c.Weight) {
-            c.Weight[to] = c.Weight[of];
+            c.Weight[to] = weight;
         }
     }
 }
