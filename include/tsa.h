@@ -391,11 +391,12 @@ int tsa_paged_append(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d
  * A cache that keeps weights gets each attended key's weight, summed over the query heads of the key head, added to weight.
  * maxCtx: host-side upper bound of ctxLens; it sizes the launch, and a sequence that turns out longer gives zeros and a bit of the
  * status word.  Value scales below 2^-100 count as zero.  The same call gives the same bits every time.
- * workspace: 16-byte aligned, not shared by calls in flight at the same time. */
+ * workspace: tsa_paged_decode_workspace_bytes(...) bytes for the same arguments (0: none needed), 16-byte aligned, not shared by calls in
+ * flight at the same time. */
 int tsa_paged_decode(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens, int nSeq,
     int maxCtx, tsa_ptr2d q, tsa_ptr2d qScale, int window, float alibiSlope, tsa_ptr2d out, int headCount, void *workspace,
     size_t workspaceBytes, int *statusWord, tsa_stream_t stream);
-size_t tsa_paged_decode_workspace_bytes(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, int nSeq, int headCount, int maxCtx);
+size_t tsa_paged_decode_workspace_bytes(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, int nSeq, int headCount, int maxCtx, int window);
 
 /* Which tokens stay when every sequence is cut to `keep` slots, for each key head by itself: the `recent` newest ones (positions above
  * tokens[s] - 1 - recent) and, of the others, the heaviest by weight; among equals the lowest slot, NaN above all numbers.  Kept tokens

@@ -147,13 +147,17 @@ LENS = [0, 1, 2, 16, 17, 33, 130, 700, 255]
     ("i8", torch.float16, 128, 32, 8, 64, 1, 0.0, torch.float16, True),
 ])
 def test_decode(kv, scale, d, heads, kvh, page, window, slope, out, track):
+    _decode_of(LENS, kv, scale, d, heads, kvh, page, window, slope, out, track)
+
+
+def _decode_of(lens, kv, scale, d, heads, kvh, page, window, slope, out, track):
     from tscale_b200 import ops
-    c = Cache(1, LENS, kvh, d, page, kv, scale, track)
-    q, qs = _query(1, len(LENS), heads, d, kv)
+    c = Cache(1, lens, kvh, d, page, kv, scale, track)
+    q, qs = _query(1, len(lens), heads, d, kv)
     before = None if c.weight is None else c.weight.clone()
     status = torch.zeros(1, dtype=torch.int32, device=DEV)
     want, added = _decode_ref(c, q, qs, heads, window, slope)
-    got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, slope, max_ctx=max(LENS), out_dtype=out, tokens=c.tokens, status=status)
+    got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, slope, max_ctx=max(lens), out_dtype=out, tokens=c.tokens, status=status)
     assert int(status) == 0
     _check_out(got, want, c)
     assert not got[0].any()
@@ -168,8 +172,97 @@ def test_decode(kv, scale, d, heads, kvh, page, window, slope, out, track):
         assert torch.equal(c.weight[~c.live].isnan(), torch.ones_like(c.weight[~c.live], dtype=torch.bool))
     # the bound may be larger than the longest sequence, and absent
     if not track:
-        assert torch.equal(got, ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, slope, max_ctx=max(LENS), out_dtype=out, tokens=c.tokens))
+        assert torch.equal(got, ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, slope, max_ctx=max(lens), out_dtype=out, tokens=c.tokens))
         _check_out(ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, slope, out_dtype=out), want, c)
+
+
+MANY = [0, 1, 700, 129, 128, 127, 2, 1000, 383, 16, 257, 640]  # with eight or more key heads: more units than clusters would have room for
+
+
+@pytest.mark.parametrize("kv,scale,d,heads,kvh,page,window,slope,out,track", [
+    ("i8", torch.float16, 128, 8, 8, 64, WHOLE, 0.0, torch.float32, False),
+    ("e4m3", torch.float16, 128, 8, 8, 16, WHOLE, 0.0, torch.float32, False),
+    ("i8", torch.float32, 64, 40, 8, 32, WHOLE, 0.01, torch.float32, True),    # five query heads per key head
+    ("e4m3", torch.float32, 64, 64, 8, 256, WHOLE, 0.0, torch.bfloat16, False),
+    ("i8", torch.float16, 128, 128, 8, 16, 300, 0.0, torch.float32, False),    # sixteen
+    ("e4m3", torch.float16, 128, 104, 8, 128, 300, 0.02, torch.float32, True),  # thirteen
+    ("i8", torch.float32, 64, 144, 8, 64, WHOLE, 0.0, torch.float32, True),    # eighteen: two units
+    ("e4m3", torch.float32, 64, 72, 4, 32, WHOLE, 0.0, torch.float16, True),
+    ("i8", torch.float16, 64, 96, 8, 64, WHOLE, 0.0, torch.float16, False),    # twelve
+])
+def test_decode_in_ranges(kv, scale, d, heads, kvh, page, window, slope, out, track):
+    _decode_of(MANY, kv, scale, d, heads, kvh, page, window, slope, out, track)
+
+
+@pytest.mark.parametrize("heads,kvh,lens", [(4, 2, [700, 300]), (16, 8, MANY), (12, 1, [513]), (128, 8, MANY)])
+@pytest.mark.parametrize("kv", ["i8", "e4m3"])
+def test_decode_logits_that_rise(heads, kvh, lens, kv):
+    """Logits that rise along the cache by about 60 powers of two: the reference moves again and again, and what was summed before fades."""
+    from tscale_b200 import ops
+    c = Cache(20, lens, kvh, 128, 32, kv, torch.float32, False)
+    q, qs = _query(20, len(lens), heads, 128, kv)
+    c.k.view(torch.int8).copy_((torch.ones_like(c.k, dtype=torch.float32) * (40 if kv == "i8" else 1)).to(c.k.dtype).view(torch.int8))
+    q = (torch.ones_like(q, dtype=torch.float32) * (40 if kv == "i8" else 1)).to(q.dtype)
+    unit = (1600 if kv == "i8" else 1) * 128 * DOT / 128 ** 0.5
+    for s, n in enumerate(lens):
+        for h in range(kvh):
+            c.write(c.ks, s, h, torch.linspace(-30, 30, max(n, 2), device=DEV)[:n] / unit)
+    qs.fill_(1.0)
+    want, _ = _decode_ref(c, q, qs, heads, WHOLE, 0.0)
+    _check_out(ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0), want, c)
+
+
+def test_decode_nan_and_bad_pages_in_ranges():
+    from tscale_b200 import ops
+    for kv in ("i8", "e4m3"):
+        c = Cache(21, [300, 290], 40, 64, 16, kv, torch.float16, False)
+        q, qs = _query(21, 2, 80, 64, kv)
+        clean = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0)
+        p, o = c.place(0)
+        for plane in (c.ks, c.vs):
+            keep = plane[p[150], 7, o[150]].clone()
+            for x in (float("nan"), float("inf")):
+                plane[p[150], 7, o[150]] = x
+                got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0)
+                assert got[0, 14 * 64:16 * 64].isnan().any(), (kv, x)
+                got[0, 14 * 64:16 * 64] = clean[0, 14 * 64:16 * 64]
+                assert torch.equal(got, clean)
+                assert not ops.paged_decode(c.kv, c.table, c.ctx, q, qs, 100, 0.0).isnan().any()  # in front of the window
+            plane[p[150], 7, o[150]] = keep
+        if kv == "e4m3":
+            c.v.view(torch.uint8)[p[150], 7, o[150]] = 0x7f
+            got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0)
+            assert got[0, 14 * 64:16 * 64].isnan().all() and torch.equal(got[1], clean[1])
+            assert not ops.paged_decode(c.kv, c.table, c.ctx, q, qs, 100, 0.0).isnan().any()
+            c.v.view(torch.uint8)[p[150], 7, o[150]] = 0
+            clean = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0)
+        for bad in (-1, c.k.shape[0], 0x7fffffff, -0x80000000):
+            table = c.table.clone()
+            table[1, 3] = bad
+            status = torch.zeros(1, dtype=torch.int32, device=DEV)
+            got = ops.paged_decode(c.kv, table, c.ctx, q, qs, WHOLE, 0.0, status=status)
+            assert int(status) != 0 and got.isfinite().all() and torch.equal(got[0], clean[0])
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0, max_ctx=295, status=status)
+        assert int(status) != 0 and not got[0].any() and float((got[1] - clean[1]).abs().max()) <= 2 * ERR * 128 * 1.5 * _unit(kv)
+
+
+def test_decode_sums_of_a_very_long_cache():
+    """Some 60 million equal keys, 1050 tiles of 128 a range, all digits of the weights and all codes at their largest: int32 sums that
+    have to be emptied on the way."""
+    from tscale_b200 import ops
+    n = 444 * 1050 * 128
+    pages = n // 256 + 1
+    shape = (pages, 1, 256)
+    k, v = torch.zeros(shape + (64,), dtype=torch.int8, device=DEV), torch.full(shape + (64,), 127, dtype=torch.int8, device=DEV)
+    scale = 0x7f7f7f / 2.0 ** 22
+    kv = ops.PagedKV(k, v, torch.ones(shape, device=DEV), torch.full(shape, scale, device=DEV))
+    ctx = torch.tensor([n + 1], dtype=torch.int32, device=DEV)
+    q = torch.ones((1, 128), dtype=torch.int8, device=DEV)
+    got = ops.paged_decode(kv, torch.arange(pages, dtype=torch.int32, device=DEV)[None], ctx, q, None, WHOLE, 0.0)
+    want = scale * 127 * n / (n + 1)
+    # a range's sums are integers below 2^24 or one rounding off; the join adds 444 records: fewer than 512 roundings of 2^-24
+    assert float((got.double() - want).abs().max()) <= 2.0 ** -15 * want
 
 
 @pytest.mark.parametrize("kv,lens,heads,kvh,d,page,track", [("i8", [20011, 3, 9999], 8, 2, 128, 64, False), ("e4m3", [30000], 3, 1, 64, 16, True),

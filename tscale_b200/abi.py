@@ -155,7 +155,7 @@ def _declare(lib):
     lib.tsa_paged_decode.argtypes = [ctypes.POINTER(PagedCfg), ctypes.POINTER(PagedKv), P, c_void_p, c_void_p, c_int, c_int, P, P, c_int, c_float, P,
                                      c_int, c_void_p, c_size_t, c_void_p, c_void_p]
     lib.tsa_paged_decode_workspace_bytes.restype = c_size_t
-    lib.tsa_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(PagedCfg), ctypes.POINTER(PagedKv), c_int, c_int, c_int]
+    lib.tsa_paged_decode_workspace_bytes.argtypes = [ctypes.POINTER(PagedCfg), ctypes.POINTER(PagedKv), c_int, c_int, c_int, c_int]
     lib.tsa_paged_evict_select.argtypes = [ctypes.POINTER(PagedKv), P, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
                                            c_void_p, c_void_p, c_void_p]
     lib.tsa_paged_evict_move.argtypes = [ctypes.POINTER(PagedCfg), ctypes.POINTER(PagedKv), P, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]

@@ -774,21 +774,35 @@ __global__ void __launch_bounds__(WGT_THREADS) PagedWeightKernel(const TPagedDec
     *reinterpret_cast<float4 *>(dst) = w;
 }
 
-// parts of the workspace, in this order
-struct TPagedWorkspace {
+// Which form a call takes.  Clusters of CTAs of two to eight tiles per warp, while at most two CTAs come to an SM, or where one CTA has a unit;
+// units that share a key head's weights leave them to the kernel behind the ranges.
+struct TPagedForm {
+    int Cluster; // CTAs of a unit; 0: ranges
+    // parts of the workspace, in this order
     size_t Partial, Lse, Logits, Bytes;
     int LogitRow;
 };
-static TPagedWorkspace PagedWorkspace(int headDim, int nSeq, int kvHeads, int headCount, int maxCtx, bool track)
+constexpr int B200_SMS = 148;
+static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, int maxCtx, int window, bool positions, bool track)
 {
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };
-    const int group = headCount / kvHeads, rows = group < PD_ROWS ? group : PD_ROWS;
-    const size_t units = (size_t)nSeq * kvHeads * ((group + PD_ROWS - 1) / PD_ROWS);
-    TPagedWorkspace w;
-    w.LogitRow = (maxCtx + PD_TILE - 1) / PD_TILE * PD_TILE;
+    const int group = headCount / kvHeads, rows = group < PD_ROWS ? group : PD_ROWS, chunks = (group + PD_ROWS - 1) / PD_ROWS;
+    const size_t units = (size_t)nSeq * kvHeads * chunks;
+    // keys of a sequence that a call looks at
+    const long long keysMax = positions ? maxCtx : window == 0 ? 1 : maxCtx < window ? maxCtx : window;
+    const long long tilesMax = (keysMax + PD_TILE - 1) / PD_TILE + 1;
+    TPagedForm w;
+    w.Cluster = 1;
+    while (w.Cluster < PD_MAX_CLUSTER && tilesMax > (PD_MIN_TILES + 1) * w.Cluster) {
+        w.Cluster *= 2;
+    }
+    if (!(tilesMax <= PD_MIN_TILES + 1 || (tilesMax <= 4 * PD_MIN_TILES * w.Cluster && units * w.Cluster <= 2 * B200_SMS)) || (track && chunks > 1)) {
+        w.Cluster = 0;
+    }
+    w.LogitRow = (int)((maxCtx < 0x7ffffff0 ? (long long)maxCtx + PD_TILE - 1 : 0x7ffffff0ll) / PD_TILE * PD_TILE);
     w.Partial = 0;
-    w.Lse = round((PD_MAX_CTAS + units) * rows * (headDim + 4) * sizeof(float));
-    w.Logits = w.Lse + (track ? round((size_t)nSeq * headCount * sizeof(float)) : 0);
+    w.Lse = w.Cluster ? 0 : round((PD_MAX_CTAS + units) * rows * (headDim + 4) * sizeof(float));
+    w.Logits = w.Lse + (track && !w.Cluster ? round((size_t)nSeq * headCount * sizeof(float)) : 0);
     w.Bytes = w.Logits + (track ? (size_t)nSeq * headCount * w.LogitRow * sizeof(float) : 0);
     return w;
 }
@@ -805,12 +819,12 @@ static const void *PickCluster(bool f16, bool wide)
 using namespace tsa;
 
 extern "C" __attribute__((visibility("default"))) size_t tsa_paged_decode_workspace_bytes(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, int nSeq, int headCount,
-    int maxCtx)
+    int maxCtx, int window)
 {
-    if (!cfg || !kv || nSeq <= 0 || kv->kv_heads <= 0 || headCount < kv->kv_heads || maxCtx < 0) {
+    if (!cfg || !kv || nSeq <= 0 || kv->kv_heads <= 0 || headCount < kv->kv_heads || maxCtx < 0 || window < 0) {
         return 0;
     }
-    return PagedWorkspace(cfg->head_dim, nSeq, kv->kv_heads, headCount, maxCtx, kv->weight != nullptr).Bytes;
+    return PagedForm(cfg->head_dim, nSeq, kv->kv_heads, headCount, maxCtx, window, kv->pos != nullptr, kv->weight != nullptr).Bytes;
 }
 
 extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable,
@@ -843,16 +857,13 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     p.Group = headCount / kv->kv_heads;
     p.HeadChunks = (p.Group + PD_ROWS - 1) / PD_ROWS;
     p.Rows = p.Group < PD_ROWS ? p.Group : PD_ROWS;
+    const bool track = kv->weight != nullptr;
     const long long room = TableTokens(p.C);
     const int longest = room < maxCtx ? (int)room : maxCtx;
-    // keys of a sequence that a call looks at
-    const long long keysMax = p.C.Pos ? longest : window == 0 ? 1 : longest < window ? longest : window;
-    const long long tilesMax = (keysMax + PD_TILE - 1) / PD_TILE + 1;
-    const long long units = (long long)nSeq * kv->kv_heads * p.HeadChunks;
+    const long long units = (long long)nSeq * kv->kv_heads * p.HeadChunks, tilesMax = (long long)longest / PD_TILE + 2;
     TSA_REQUIRE(units * tilesMax < (1ll << 31), "tsa_paged_decode: %d sequences of %d tokens with %d query heads are too much for one call", nSeq, longest, headCount);
-    const bool track = kv->weight != nullptr;
-    const TPagedWorkspace ws = PagedWorkspace(D, nSeq, kv->kv_heads, headCount, maxCtx, track);
-    TSA_REQUIRE(workspace && workspaceBytes >= ws.Bytes, "tsa_paged_decode: workspace of %zu bytes needed, %zu given", ws.Bytes, workspaceBytes);
+    const TPagedForm form = PagedForm(D, nSeq, kv->kv_heads, headCount, maxCtx, window, kv->pos != nullptr, track);
+    TSA_REQUIRE(form.Bytes == 0 || (workspace && workspaceBytes >= form.Bytes), "tsa_paged_decode: workspace of %zu bytes needed, %zu given", form.Bytes, workspaceBytes);
     TSA_REQUIRE((uintptr_t)workspace % 16 == 0, "tsa_paged_decode: workspace must be 16-byte aligned");
     p.CtxLens = ctxLens;
     p.Tokens = tokens;
@@ -868,35 +879,23 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     p.QScale = P2D<float>(qScale);
     p.Out = P2D<char>(out);
     p.Partial = (float *)workspace;
-    p.Lse = track ? (float *)((char *)workspace + ws.Lse) : nullptr;
-    p.Logits = track ? (float *)((char *)workspace + ws.Logits) : nullptr;
-    p.LogitRow = ws.LogitRow;
+    p.Lse = track ? (float *)((char *)workspace + form.Lse) : nullptr;
+    p.Logits = track ? (float *)((char *)workspace + form.Logits) : nullptr;
+    p.LogitRow = form.LogitRow;
     p.Status = statusWord;
-    const bool wide = p.Group > 8, e4m3 = cfg->kv_dtype == TSA_E4M3, f16 = cfg->scale_dtype == TSA_F16;
+    p.Cluster = form.Cluster;
+    const bool e4m3 = cfg->kv_dtype == TSA_E4M3, f16 = cfg->scale_dtype == TSA_F16;
     p.ScaleF16 = f16;
-    int dev = 0, sms = 0;
-    rc = CheckCuda(cudaGetDevice(&dev), "cudaGetDevice");
-    if (rc == TSA_OK) {
-        rc = CheckCuda(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
-    }
-    if (rc != TSA_OK) {
-        return rc;
-    }
     cudaStream_t s = (cudaStream_t)stream;
-    // clusters of CTAs of two to eight tiles per warp, while at most two CTAs come to an SM; units that share a key head's weights leave
-    // them to the second kernel of the ranges
-    p.Cluster = 1;
-    while (p.Cluster < PD_MAX_CLUSTER && tilesMax > (PD_MIN_TILES + 1) * p.Cluster) {
-        p.Cluster *= 2;
-    }
-    if ((p.Cluster == 1 || (tilesMax <= 4 * PD_MIN_TILES * p.Cluster && units * p.Cluster <= 2ll * sms)) && !(track && p.HeadChunks > 1)) {
+    if (form.Cluster) {
+        const bool wide = p.Group > 8;
         const void *kern = D == 128 ? (e4m3 ? PickCluster<128, true>(f16, wide) : PickCluster<128, false>(f16, wide))
                                     : (e4m3 ? PickCluster<64, true>(f16, wide) : PickCluster<64, false>(f16, wide));
         void *args[] = {&p};
         return CheckCuda(LaunchPdl(kern, dim3((unsigned)(units * p.Cluster)), dim3(PD_THREADS), 0, s, args, p.Cluster), "tsa_paged_decode launch");
     }
     unsigned ctas = 0;
-    rc = LaunchPagedRanges(p, kv, D, e4m3, keysMax / PD_RANGE_TILE + 2, &ctas, s);
+    rc = LaunchPagedRanges(p, kv, D, e4m3, (long long)(p.C.Pos || longest < window ? longest : window) / PD_RANGE_TILE + 2, &ctas, s);
     if (rc == TSA_OK) {
         const void *join = D == 128 ? (const void *)PagedJoinKernel<128> : (const void *)PagedJoinKernel<64>;
         bool byUnit = units * 4 < ctas;

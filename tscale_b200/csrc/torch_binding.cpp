@@ -625,11 +625,13 @@ PyObject *PagedDecode(PyObject *, PyObject *const *a, Py_ssize_t n)
         const c10::cuda::CUDAGuard guard(p.First().device());
         const at::Tensor out = given ? *given : Empty(p.NSeq, (int64_t)heads * p.Cfg.head_dim, TorchType(p.Cfg.out_dtype), q);
         const tsa_ptr2d o2 = P2D(out);
-        const at::Tensor space = ws ? *ws : EmptyBytes(g.PagedDecodeWs(&p.Cfg, &p.Kv, p.NSeq, heads, maxCtx), q);
+        const size_t need = ws ? 0 : g.PagedDecodeWs(&p.Cfg, &p.Kv, p.NSeq, heads, maxCtx, window);
+        const at::Tensor space = ws ? *ws : need ? EmptyBytes(need, q) : at::Tensor();
+        void *const spacePtr = space.defined() ? space.data_ptr() : nullptr;
         tsa_stream_t stream = Stream();
         const int rc = Unlocked([&] {
-            return g.PagedDecode(&p.Cfg, &p.Kv, p.Table, p.LensPtr(), p.TokensPtr(), p.NSeq, maxCtx, q2, qs2, window, slope, o2, heads, space.data_ptr(),
-                (size_t)space.nbytes(), status ? (int *)status->data_ptr() : nullptr, stream);
+            return g.PagedDecode(&p.Cfg, &p.Kv, p.Table, p.LensPtr(), p.TokensPtr(), p.NSeq, maxCtx, q2, qs2, window, slope, o2, heads, spacePtr,
+                space.defined() ? (size_t)space.nbytes() : 0, status ? (int *)status->data_ptr() : nullptr, stream);
         });
         return Result(rc, out);
     });
