@@ -389,24 +389,26 @@ __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM :
     // one more in the bin of each order that is in: (order >> shift) & low; equal bins of a whole step (weights that are all zero) are one addition
     auto count = [&](unsigned *hist, const uint4 &o, int shift, unsigned low, unsigned in) {
         const unsigned x = o.x >> shift & low, y = o.y >> shift & low, z = o.z >> shift & low, w = o.w >> shift & low;
-        const unsigned first = __shfl_sync(0xffffffffu, x, 0);
-        if (__all_sync(0xffffffffu, in == 15 && x == first && y == first && z == first && w == first)) {
-            if (lane == 0) {
-                atomicAdd(hist + first, 128);
+        if (__all_sync(0xffffffffu, in == 15 && x == y && x == z && x == w)) {
+            const unsigned first = __shfl_sync(0xffffffffu, x, 0);
+            if (__all_sync(0xffffffffu, x == first)) {
+                if (lane == 0) {
+                    atomicAdd(hist + first, 128);
+                }
+                return;
             }
-        } else {
-            if (in & 1) {
-                atomicAdd(hist + x, 1);
-            }
-            if (in & 2) {
-                atomicAdd(hist + y, 1);
-            }
-            if (in & 4) {
-                atomicAdd(hist + z, 1);
-            }
-            if (in & 8) {
-                atomicAdd(hist + w, 1);
-            }
+        }
+        if (in & 1) {
+            atomicAdd(hist + x, 1);
+        }
+        if (in & 2) {
+            atomicAdd(hist + y, 1);
+        }
+        if (in & 4) {
+            atomicAdd(hist + z, 1);
+        }
+        if (in & 8) {
+            atomicAdd(hist + w, 1);
         }
     };
     // of four slots from s on, the ones below `limit`
@@ -455,13 +457,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM :
         constexpr int SHIFT[3] = {21, 10, 0};
         constexpr unsigned low = 1023;
         if (digit == 1) {
+#pragma unroll 2
             for (int s0 = beg; s0 < end; s0 += 128) {
                 const int s = s0 + 4 * lane;
                 const uint4 o4 = s < end ? orders(s) : make_uint4(0, 0, 0, 0);
                 const unsigned in = until(s, end) & agree(o4, 0xffe00000u, cut);
-                if (__any_sync(0xffffffffu, in)) {
+                if (in) {
                     const unsigned o[4] = {o4.x, o4.y, o4.z, o4.w};
-                    int at = in ? atomicAdd(&sh.ListLen, __popc(in)) : 0;
+                    int at = atomicAdd(&sh.ListLen, __popc(in));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (in >> i & 1) {
@@ -471,8 +474,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM :
                             ++at;
                         }
                     }
-                    count(sh.Hist[1], o4, 10, 2047, in);
                 }
+                count(sh.Hist[1], o4, 10, 2047, in);
             }
         } else if (digit == 2) {
             if (sh.ListLen <= SEL_LIST) {
@@ -560,9 +563,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM :
         const uint4 o = orders(s & ~3);
         return s & 2 ? (s & 1 ? o.w : o.z) : (s & 1 ? o.y : o.x);
     };
-    // whether slot s stays; `left`: of the ties
-    auto kept = [&](int s, int &left) {
-        const unsigned o = s < end ? order(s) : 0;
+    // whether slot s, of order o, stays; `left`: of the ties
+    auto kept = [&](int s, unsigned o, int &left) {
         bool k = s < end && o >= cut;
         if (!allTies) {
             const unsigned tie = __ballot_sync(0xffffffffu, k && o == cut);
@@ -573,11 +575,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM :
     };
     // slots that leave a hole in front of the budget, or that are moved from behind it
     int hole = 0, mover = 0, left = ties;
-    for (int s0 = beg; s0 < end; s0 += 32) {
-        const int s = s0 + lane;
-        const bool k = kept(s, left);
-        hole += s < p.Keep && s < end && !k;
-        mover += s >= p.Keep && k;
+    for (int s0 = beg; s0 < end; s0 += 128) {
+        unsigned o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int s = s0 + 32 * j + lane;
+            o[j] = s < end ? order(s) : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int s = s0 + 32 * j + lane;
+            const bool k = kept(s, o[j], left);
+            hole += s < p.Keep && s < end && !k;
+            mover += s >= p.Keep && k;
+        }
     }
     hole = __reduce_add_sync(0xffffffffu, hole);
     mover = __reduce_add_sync(0xffffffffu, mover);
@@ -607,25 +618,53 @@ __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM :
     }
     // (as many of each as there is room for: at most min(keep, len - keep))
     left = ties;
-    for (int s0 = beg; s0 < end; s0 += 32) {
-        const int s = s0 + lane;
-        const bool k = kept(s, left);
-        if (s0 < p.Keep) {
-            const bool is = s < p.Keep && s < end && !k;
-            const unsigned all = __ballot_sync(0xffffffffu, is);
-            if (is) {
-                moves[hole + __popc(all & below)].x = s;
-            }
-            hole += __popc(all);
+    for (int s0 = beg; s0 < end; s0 += 128) {
+        unsigned o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int s = s0 + 32 * j + lane;
+            o[j] = s < end ? order(s) : 0;
         }
-        if (s0 + 32 > p.Keep) {
-            const bool is = s >= p.Keep && k;
-            const unsigned all = __ballot_sync(0xffffffffu, is);
-            if (is) {
-                moves[mover + __popc(all & below)].y = s;
+        if (s0 < p.Keep && s0 + 128 > p.Keep) {
+            // the budget ends in this step
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+                const int s = s0 + 32 * j + lane;
+                const bool k = kept(s, s < end ? order(s) : 0, left), isHole = s < p.Keep && s < end && !k, isMover = s >= p.Keep && k;
+                const unsigned holes = __ballot_sync(0xffffffffu, isHole), movers = __ballot_sync(0xffffffffu, isMover);
+                if (isHole) {
+                    moves[hole + __popc(holes & below)].x = s;
+                }
+                if (isMover) {
+                    moves[mover + __popc(movers & below)].y = s;
+                }
+                hole += __popc(holes);
+                mover += __popc(movers);
             }
-            mover += __popc(all);
+            continue;
         }
+        // all in front of it or all behind it
+        const bool front = s0 < p.Keep;
+        int *const dst = front ? &moves[0].x : &moves[0].y;
+        int &sofar = front ? hole : mover;
+        unsigned which[4];
+        bool is[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int s = s0 + 32 * j + lane;
+            const bool k = kept(s, o[j], left);
+            is[j] = front ? s < end && !k : k;
+            which[j] = __ballot_sync(0xffffffffu, is[j]);
+        }
+        int at = sofar;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (is[j]) {
+                dst[2 * (at + __popc(which[j] & below))] = s0 + 32 * j + lane;
+            }
+            at += __popc(which[j]);
+        }
+        sofar = at;
     }
     for (int i = moved + rank * THREADS + tid; i < p.MoveCap; i += p.Cluster * THREADS) {
         moves[i] = make_int2(-1, -1);
