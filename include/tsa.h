@@ -352,7 +352,8 @@ size_t tsa_att_decode_static_capacity_bytes(void);
  * all contiguous, in device memory, 16-byte aligned.  Slot t of sequence s is slot t % page_size of page pageTable[s][t / page_size]
  * (int32 [nSeq][maxPages], device memory; entries behind a sequence's last page are not read).  ctxLens[s] (device) is the number of
  * slots that the sequence fills; tokens[s] (device; NULL without pos) the number of tokens that it has seen, so that its newest token
- * has position tokens[s] - 1 (ctxLens[s] - 1 without pos).
+ * has position tokens[s] - 1 (ctxLens[s] - 1 without pos).  A row of the table has room for 2^30 tokens at most.  Sequences may share
+ * pages (of a common beginning, say) where no call writes to them: append and evict_move write, and so does decode to weight.
  * A page number outside the pool, or a length beyond the table's or the caller's bound, sets a bit of the status word; the rows
  * concerned are not stored, attended, chosen or moved, and nothing outside the buffers is touched. */
 typedef struct {

@@ -498,6 +498,38 @@ def test_select(lens, kvh, page, keep, recent, positions, values):
             assert moves[s, h].tolist() == [list(m) for m in want] + [[-1, -1]] * (moves.shape[2] - len(want))
 
 
+def test_select_in_two_threads():
+    """Calls of different sizes at once: the launch of each finds the shared memory it asks for."""
+    import threading
+    from tscale_b200 import ops
+    jobs, wrong = [], []
+    for seed, (n, length) in enumerate([(200, 12000), (2, 5000), (1, 70000)]):
+        pages = n * -(-length // 64)
+        weight = torch.rand((pages, 1, 64), generator=_gen(seed), device=DEV)
+        table = torch.arange(pages, dtype=torch.int32, device=DEV).view(n, -1)
+        kv = ops.PagedKV(None, None, None, None, None, weight)
+        call = lambda kv=kv, table=table, ctx=torch.full((n,), length, dtype=torch.int32, device=DEV): ops.paged_evict_select(kv, table, ctx, 900, 10)  # noqa: E731
+        jobs.append((call, call()))
+
+    def work(call, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(150):
+                    got = call()
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except Exception as e:
+            wrong.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=jobs[i % 3]) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[0]
+
+
 @pytest.mark.parametrize("kv,scale,kvh,d,page,track", [("i8", torch.float16, 3, 128, 16, True), ("e4m3", torch.float32, 2, 64, 64, True),
                                                        ("i8", torch.float32, 1, 128, 32, False)])
 def test_move(kv, scale, kvh, d, page, track):

@@ -48,7 +48,7 @@ def _move(cfg=None, kv=None, moves=FAKE, cap=5, counts=FAKE, n=3):
 
 
 POOLS = [(dict(page_size=48), b"page size"), (dict(page_size=8), b"page size"), (dict(page_size=512), b"page size"), (dict(page_count=0), b"pages"),
-         (dict(kv_heads=0), b"pages"), (dict(page_count=1 << 20, kv_heads=1 << 12), b"pages"), (dict(k=None), b"null"), (dict(v_scale=None), b"null"),
+         (dict(kv_heads=0), b"pages"), (dict(page_count=1 << 20, kv_heads=1 << 12), b"pages"), (dict(kv_heads=65536), b"key heads"), (dict(k=None), b"null"), (dict(v_scale=None), b"null"),
          (dict(k=FAKE + 8), b"aligned"), (dict(pos=FAKE + 4), b"aligned")]
 
 
@@ -66,7 +66,7 @@ def test_types_that_are_refused(kw):
 
 @pytest.mark.parametrize("call,kw,text", [
     (_append, dict(n=-1), b"sequences"), (_append, dict(n=70000), b"sequences"), (_append, dict(table=NULL), b"page table"), (_append, dict(ctx=None), b"page table"),
-    (_append, dict(table=_plane(4, 2)), b"page table"), (_append, dict(table=_plane(4, 3, stride=18)), b"page table"), (_append, dict(rows=-1), b"row count"),
+    (_append, dict(table=_plane(4, 2)), b"page table"), (_append, dict(table=_plane((1 << 24) + 1, 3)), b"2^30"), (_append, dict(table=_plane(4, 3, stride=18)), b"page table"), (_append, dict(rows=-1), b"row count"),
     (_append, dict(starts=None), b"rowStarts"), (_append, dict(k=abi.Ptr2D(FAKE, 128, 100, 5)), b"extents"), (_append, dict(k=abi.Ptr2D(FAKE, 128, 128, 4)), b"extents"),
     (_append, dict(k=abi.Ptr2D(FAKE + 8, 128, 128, 5)), b"aligned"), (_append, dict(k=abi.Ptr2D(FAKE, 136, 128, 5)), b"aligned"),
     (_append, dict(ks=_plane(4, 2)), b"kvHeads"), (_append, dict(ks=_plane(5, 1)), b"kvHeads"), (_append, dict(ks=_plane(5, 2, stride=22)), b"aligned"),
@@ -131,6 +131,11 @@ def test_other_arguments_that_are_refused():
                      ((TABLE, CTX, torch.zeros((3, 100), dtype=torch.int8), None, 5, 0.0), {}), ((TABLE, CTX, q, None, 5, 0.0), {})):  # the last: not on a GPU
         with pytest.raises(AssertionError):
             ops.paged_decode(kv, *args, **kw)
+    for kw in (dict(max_ctx=1 << 32), dict(max_ctx=-1 << 40)):  # would be another number in 32 bits
+        with pytest.raises(AssertionError, match="32 bits"):
+            ops.paged_decode(kv, TABLE, CTX, q, None, 5, 0.0, tokens=CTX, **kw)
+        with pytest.raises(AssertionError, match="32 bits"):
+            ops.paged_evict_select(kv, TABLE, CTX, 5, 1, tokens=CTX, **kw)
     with pytest.raises(TypeError):
         ops.paged_decode(kv[:5], TABLE, CTX, q, None, 5, 0.0)
     for args in ((row, scale.half(), row, scale), (row.to(torch.uint8), scale, row, scale), (row, scale, row, scale)):

@@ -28,9 +28,12 @@ int CheckPages(const char *fn, const tsa_paged_cfg *cfg, const tsa_paged_kv *kv,
     TSA_REQUIRE(kv->page_size == 1 << shift, "%s: page size %d must be 16, 32, 64, 128 or 256", fn, kv->page_size);
     TSA_REQUIRE(kv->page_count > 0 && kv->kv_heads > 0 && (long long)kv->page_count * kv->kv_heads <= 0x7fffffff, "%s: %d pages of %d key heads", fn,
         kv->page_count, kv->kv_heads);
+    TSA_REQUIRE(kv->kv_heads <= 65535, "%s: %d key heads (at most 65535)", fn, kv->kv_heads);
     TSA_REQUIRE(nSeq >= 0 && nSeq <= 65535, "%s: %d sequences (at most 65535)", fn, nSeq);
     TSA_REQUIRE(nSeq == 0 || (pageTable.data && ctxLens), "%s: null page table or ctxLens", fn);
     TSA_REQUIRE(nSeq == 0 || (pageTable.ysize >= nSeq && pageTable.xsize > 0), "%s: page table smaller than [nSeq][1]", fn);
+    TSA_REQUIRE(nSeq == 0 || (long long)pageTable.xsize << shift <= 1 << 30, "%s: a page table of %d columns has room for more than 2^30 tokens of a sequence", fn,
+        pageTable.xsize);
     TSA_REQUIRE((uintptr_t)pageTable.data % 4 == 0 && pageTable.stride_bytes % 4 == 0, "%s: the page table must be 4-byte aligned", fn);
     TPages &c = *res;
     c.K = (uint8_t *)kv->k;
@@ -875,8 +878,8 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_evict_select(con
     const void *kern = many ? (cached ? (const void *)PagedSelectKernel<1024, true> : (const void *)PagedSelectKernel<1024, false>)
                             : (const void *)PagedSelectKernel<SEL_THREADS, true>;
     const size_t smem = cached ? (size_t)slice * sizeof(unsigned) : 0;
-    if (smem > 8 * 1024) { // beyond 48 KB with the counts
-        rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute");
+    if (smem > 8 * 1024) { // beyond 48 KB with the counts.  The same limit in every call: another thread's may come between this and the launch
+        rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_SLICE * sizeof(unsigned)), "cudaFuncSetAttribute");
         if (rc != TSA_OK) {
             return rc;
         }
@@ -895,7 +898,6 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_evict_move(const
         return rc;
     }
     TSA_REQUIRE(moveCap >= 0, "tsa_paged_evict_move: negative moveCap");
-    TSA_REQUIRE(kv->kv_heads <= 65535, "tsa_paged_evict_move: %d key heads (at most 65535)", kv->kv_heads);
     if (nSeq == 0 || moveCap == 0) {
         return TSA_OK;
     }

@@ -501,6 +501,13 @@ int Size(int64_t n)
     return (int)n;
 }
 
+int Int32(PyObject *o)
+{
+    const long v = Int(o);
+    Need(v >= -0x7fffffff - 1 && v <= 0x7fffffff, PyExc_AssertionError, "number beyond 32 bits");
+    return (int)v;
+}
+
 void SameGpu(const at::Tensor &first, std::initializer_list<const at::Tensor *> others)
 {
     bool ok = first.is_cuda();
@@ -616,8 +623,8 @@ PyObject *PagedDecode(PyObject *, PyObject *const *a, Py_ssize_t n)
         const at::Tensor *qs = Tensor(a[6]), *given = Tensor(a[11]), *ws = Tensor(a[12]), *status = Tensor(a[13]);
         const tsa_ptr2d q2 = p.Codes(q), qs2 = Plane(qs, at::kFloat, "expected float32 query scales");
         Need(p.Cfg.head_dim > 0 && q2.xsize % p.Cfg.head_dim == 0, PyExc_AssertionError, "expected queries [sequences][heads * head size]");
-        const int heads = q2.xsize / p.Cfg.head_dim, window = (int)Int(a[8]);
-        const int maxCtx = a[4] == Py_None ? Size((int64_t)p.Table.xsize * p.Kv.page_size) : (int)Int(a[4]);
+        const int heads = q2.xsize / p.Cfg.head_dim, window = Int32(a[8]);
+        const int maxCtx = a[4] == Py_None ? Size((int64_t)p.Table.xsize * p.Kv.page_size) : Int32(a[4]);
         const float slope = Float(a[9]);
         p.Cfg.qk_vec_scale = Float(a[7]);
         p.Cfg.out_dtype = given ? TsaType(*given) : (int)Int(a[10]);
@@ -643,10 +650,10 @@ PyObject *PagedEvictSelect(PyObject *, PyObject *const *a, Py_ssize_t n)
     return Guard<8>(n, [&] {
         const TPaged p(a[0], a[1], a[2], a[3], false);
         const at::Tensor *status = Tensor(a[7]);
-        const int maxCtx = a[4] == Py_None ? Size((int64_t)p.Table.xsize * p.Kv.page_size) : (int)Int(a[4]), keep = (int)Int(a[5]), recent = (int)Int(a[6]);
+        const int maxCtx = a[4] == Py_None ? Size((int64_t)p.Table.xsize * p.Kv.page_size) : Int32(a[4]), keep = Int32(a[5]), recent = Int32(a[6]);
         p.OneGpu({status});
         const c10::cuda::CUDAGuard guard(p.First().device());
-        const int cap = std::max(1, std::min(keep, maxCtx - keep));
+        const int cap = (int)std::max<int64_t>(1, std::min<int64_t>(keep, (int64_t)maxCtx - keep));
         const at::TensorOptions ints = at::TensorOptions().dtype(at::kInt).device(p.First().device());
         const at::Tensor moves = at::empty({p.NSeq, p.Kv.kv_heads, cap, 2}, ints), counts = at::empty({p.NSeq, p.Kv.kv_heads}, ints), lens = at::empty({p.NSeq}, ints);
         tsa_stream_t stream = Stream();
