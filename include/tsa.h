@@ -391,7 +391,7 @@ int tsa_paged_append(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d
  * absent), out [nSeq][headCount * D] of out_dtype.  Sequences without keys give zeros.
  * A cache that keeps weights gets each attended key's weight, summed over the query heads of the key head, added to weight.
  * maxCtx: host-side upper bound of ctxLens; it sizes the launch, and a sequence that turns out longer gives zeros and a bit of the
- * status word.  Value scales below 2^-100 count as zero.  The same call gives the same bits every time.
+ * status word.  Value scales below 2^-80 may count as zero.  The same call gives the same bits every time.
  * workspace: tsa_paged_decode_workspace_bytes(...) bytes for the same arguments (0: none needed), 16-byte aligned, not shared by calls in
  * flight at the same time. */
 int tsa_paged_decode(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens, int nSeq,

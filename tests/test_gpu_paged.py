@@ -308,6 +308,27 @@ def test_decode_scales_of_any_size():
     _check_out(ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0), want, c)
 
 
+@pytest.mark.parametrize("kv", ["i8", "e4m3"])
+def test_decode_values_that_are_all_zero(kv):
+    """Four million keys of value scale zero, the logits of every other tile higher by 7.9: nothing to add up, but their weights count."""
+    from tscale_b200 import ops
+    n = 444 * 80 * 128
+    shape = (n // 256 + 1, 1, 256)
+    codes = [torch.ones(shape + (64,), device=DEV).to(CODES[kv]) for _ in range(2)]
+    ks = torch.full(shape, 50.0 / 8 / DOT, device=DEV)
+    ks[:, :, 128:] = 57.9 / 8 / DOT
+    cache = ops.PagedKV(*codes, ks, torch.zeros(shape, device=DEV), None, torch.zeros(shape, device=DEV))
+    table, ctx = torch.arange(shape[0], dtype=torch.int32, device=DEV)[None], torch.tensor([n + 1], dtype=torch.int32, device=DEV)
+    got = ops.paged_decode(cache, table, ctx, torch.ones((1, 128), device=DEV).to(CODES[kv]), None, WHOLE, 0.0)
+    assert not got.any()
+    # The heavier half has weight 2 / (n / 2 * (1 + 2^-7.9)) for two heads; the sink, 2^-57, is below all roundings.  Exponents: z - reference
+    # and the logarithm of the sum are below 129, each half a step of 2^-16 off, the results of three more additions less than that again; times
+    # ln 2 that is below 2^-15.  Sums: 80 + 8 + 444 additions of 2^-24.  The lighter half's own logits count 2^-7.9 times
+    w = cache.weight.view(-1)[:n].view(-1, 256)
+    assert float((w[:, 128:].double() * (n / 4 * (1 + 2 ** -7.9)) - 1).abs().max()) <= 2.0 ** -14 + 2.0 ** -15
+    assert float((w[:, :128].double() * (n / 4 * (1 + 2 ** 7.9)) - 1).abs().max()) <= 2.0 ** -13
+
+
 def test_decode_nan_and_infinity_stay_where_they_are():
     from tscale_b200 import ops
     c = Cache(5, [200, 90], 2, 64, 16, "e4m3", torch.float16, False)
