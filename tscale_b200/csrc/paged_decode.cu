@@ -774,15 +774,21 @@ __global__ void __launch_bounds__(WGT_THREADS) PagedWeightKernel(const TPagedDec
     *reinterpret_cast<float4 *>(dst) = w;
 }
 
-// Which form a call takes.  Clusters of CTAs of two to eight tiles per warp, while at most two CTAs come to an SM, or where one CTA has a unit;
-// units that share a key head's weights leave them to the kernel behind the ranges.
+// Which form a call takes.  Clusters of CTAs of two to eight tiles per warp while all of them are resident (four to an SM, three where more than
+// eight heads share a key head; of eight CTAs, which have to lie in one part of the chip, on 128 of the SMs), with fewer CTAs of a unit where that
+// makes them so.  Measured, in us, as clusters and as ranges, for units of two int8 heads of 128 dimensions (8 key heads a sequence):
+//   units x slots      8 x 256    64 x 1024   64 x 4000   72 x 1024 (of 4)  128 x 512   256 x 256   256 x 1024 (of 2: left to the ranges)
+//   clusters / ranges  5.5 / 6.6  7.4 / 9.1   14.9 / 15.4     9.0 / 9.7     7.6 / 9.7   7.4 / 8.8   26.9 / 15.8
+// Beyond the resident ones a CTA per unit pays while it has few tiles, 16 (8 for more than eight heads): 1024 units of 128 slots 12.4 / 16.9, of
+// 256 slots 17.0 / 20.9, of 512 slots 31.0 / 32.0, 2048 units of 512 slots 58 / 54.
+// Units that share a key head's weights leave them to the kernel behind the ranges.
 struct TPagedForm {
     int Cluster; // CTAs of a unit; 0: ranges
     // parts of the workspace, in this order
     size_t Partial, Lse, Logits, Bytes;
     int LogitRow;
 };
-constexpr int B200_SMS = 148;
+constexpr int B200_SMS = 148, PD_MAX_CLUSTER_SMS = 128;
 static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, int maxCtx, int window, bool positions, bool track)
 {
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };
@@ -796,7 +802,12 @@ static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, i
     while (w.Cluster < PD_MAX_CLUSTER && tilesMax > (PD_MIN_TILES + 1) * w.Cluster) {
         w.Cluster *= 2;
     }
-    if (!(tilesMax <= PD_MIN_TILES + 1 || (tilesMax <= 4 * PD_MIN_TILES * w.Cluster && units * w.Cluster <= 2 * B200_SMS)) || (track && chunks > 1)) {
+    auto resident = [&] { return units * w.Cluster <= (size_t)(w.Cluster == PD_MAX_CLUSTER ? PD_MAX_CLUSTER_SMS : B200_SMS) * (rows > 8 ? 3 : 4); };
+    while (w.Cluster > 1 && !resident()) {
+        w.Cluster /= 2;
+    }
+    const bool inTime = resident() && tilesMax <= 4 * PD_MIN_TILES * w.Cluster, one = w.Cluster == 1 && tilesMax <= PD_MIN_TILES * (rows > 8 ? 1 : 2) + 1;
+    if (!(inTime || one) || (track && chunks > 1)) {
         w.Cluster = 0;
     }
     w.LogitRow = (int)((maxCtx < 0x7ffffff0 ? (long long)maxCtx + PD_TILE - 1 : 0x7ffffff0ll) / PD_TILE * PD_TILE);
