@@ -697,6 +697,12 @@ int LaunchPagedRanges(const TPagedDecodeParams &p, const tsa_paged_kv *kv, int h
     *ctas = *ctas < PD_MAX_CTAS ? *ctas : PD_MAX_CTAS;
     TPagedDecodeParams copy = p;
     void *args[] = {&tmK, &tmV, &copy};
+    // Three CTAs to an SM find no place on some while the kernel before is still there, and the ones left over run alone at the end: with eight
+    // tiles each or more they rather come when it has gone (64 dimensions, 512 key heads of 2000 .. 6000 slots: 66 us, and 57.6 this way; five tiles each,
+    // 64 of 4100: 13.4 and 14.8; two CTAs to an SM, 128 dimensions, 8 of 100000 .. 131072: 49.3 and 51.5)
+    if (perSm > 2 && total >= 8ll * *ctas) {
+        return CheckCuda(cudaLaunchKernel(kern, dim3(*ctas), dim3(PT_THREADS), args, smem, stream), "tsa_paged_decode launch");
+    }
     return CheckCuda(LaunchPdl(kern, dim3(*ctas), dim3(PT_THREADS), smem, stream, args), "tsa_paged_decode launch");
 }
 
