@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     constexpr int KS = E4M3 ? D / 16 : D / 32;      // steps of the score product
     constexpr int ROWS = 8 * HALVES;
     typedef typename std::conditional<D == 128, uint4, uint2>::type TPiece; // D / 8 dimensions of a key
+    extern __shared__ __align__(16) float logits[]; // of this CTA's keys, [rows][p.LogitRow]
     __shared__ __align__(16) float accOf[PD_WARPS][ROWS][D + 4]; // [.][.][16 j + 2 g + b] for dimension D / 8 g + 2 j + b: no two lanes of a store meet in a bank
     __shared__ float refOf[PD_WARPS][ROWS], sumOf[PD_WARPS][ROWS], ctaRef[ROWS], ctaSum[ROWS], lseOf[ROWS], factorOf[ROWS][PD_MAX_CLUSTER];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     const int keyBeg = keys.Beg, keyEnd = min(keys.End, segEnd * PD_TILE);
     const int nearest = p.Window > 0 ? 1 : 0;
     const unsigned spread = p.Window > 0 ? p.Window : 1;
-    float *const logits = p.Logits ? p.Logits + ((size_t)seq * p.HeadCount + firstHead) * p.LogitRow : nullptr;
+    const bool track = c.Weight != nullptr;
 
     // the query heads of this lane's rows, in the dimensions' order of the fragments
     uint32_t qa[KS][4];
@@ -350,11 +351,11 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
                         }
                     }
                 }
-                if (logits && tile + u < segEnd) {
+                if (track && tile + u < segEnd) {
 #pragma unroll
                     for (int half = 0; half < HALVES; ++half) {
                         if (g + 8 * half < rows) {
-                            *reinterpret_cast<float4 *>(logits + (size_t)(g + 8 * half) * p.LogitRow + key0) =
+                            *reinterpret_cast<float4 *>(logits + (g + 8 * half) * p.LogitRow + key0 - segBeg * PD_TILE) =
                                 make_float4(z[u][half][0], z[u][half][1], z[u][half][2], z[u][half][3]);
                         }
                     }
@@ -558,7 +559,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
         }
         StoreFromFloat(p.Out.Row(seq), (firstHead + r) * D + d, p.OutDtype, a);
     }
-    if (logits) {
+    if (track) {
         // the weights of this CTA's keys (one unit per key head: nobody else adds to them)
         for (int key = max(keyBeg, segBeg * PD_TILE) + tid; key < keyEnd; key += PD_THREADS) {
             const int page = table[key >> c.PageShift];
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
                 float w = 0;
 #pragma unroll 4
                 for (int r = 0; r < rows; ++r) {
-                    w += Exp2(logits[(size_t)r * p.LogitRow + key] - lseOf[r]);
+                    w += Exp2(logits[r * p.LogitRow + key - segBeg * PD_TILE] - lseOf[r]);
                 }
                 c.Weight[PlaneSlot(c, page, head) + (key & ((1 << c.PageShift) - 1))] += w;
             }
@@ -812,11 +813,16 @@ static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, i
     if (!(inTime || one) || (track && chunks > 1)) {
         w.Cluster = 0;
     }
-    w.LogitRow = (int)((maxCtx < 0x7ffffff0 ? (long long)maxCtx + PD_TILE - 1 : 0x7ffffff0ll) / PD_TILE * PD_TILE);
+    // clusters: of a CTA, an odd number of tiles, so that the rows of a store lie in different banks
+    w.LogitRow = w.Cluster ? (int)((tilesMax + w.Cluster - 1) / w.Cluster | 1) * PD_TILE
+                           : (int)((maxCtx < 0x7ffffff0 ? (long long)maxCtx + PD_TILE - 1 : 0x7ffffff0ll) / PD_TILE * PD_TILE);
     w.Partial = 0;
-    w.Lse = w.Cluster ? 0 : round((PD_MAX_CTAS + units) * rows * (headDim + 4) * sizeof(float));
-    w.Logits = w.Lse + (track && !w.Cluster ? round((size_t)nSeq * headCount * sizeof(float)) : 0);
-    w.Bytes = w.Logits + (track ? (size_t)nSeq * headCount * w.LogitRow * sizeof(float) : 0);
+    w.Lse = w.Logits = w.Bytes = 0; // a cluster has all it needs in shared memory
+    if (!w.Cluster) {
+        w.Lse = round((PD_MAX_CTAS + units) * rows * (headDim + 4) * sizeof(float));
+        w.Logits = w.Lse + (track ? round((size_t)nSeq * headCount * sizeof(float)) : 0);
+        w.Bytes = w.Logits + (track ? (size_t)nSeq * headCount * w.LogitRow * sizeof(float) : 0);
+    }
     return w;
 }
 
@@ -904,8 +910,16 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
         const bool wide = p.Group > 8;
         const void *kern = D == 128 ? (e4m3 ? PickCluster<128, true>(f16, wide) : PickCluster<128, false>(f16, wide))
                                     : (e4m3 ? PickCluster<64, true>(f16, wide) : PickCluster<64, false>(f16, wide));
+        const size_t smem = track ? p.Rows * form.LogitRow * sizeof(float) : 0;
+        if (smem > 0 && wide) { // beyond 48 KB with what the kernel has anyway; the same limit in every call
+            rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PD_ROWS * (4 * PD_MIN_TILES + 1) * PD_TILE * sizeof(float)),
+                "cudaFuncSetAttribute");
+            if (rc != TSA_OK) {
+                return rc;
+            }
+        }
         void *args[] = {&p};
-        return CheckCuda(LaunchPdl(kern, dim3((unsigned)(units * p.Cluster)), dim3(PD_THREADS), 0, s, args, p.Cluster), "tsa_paged_decode launch");
+        return CheckCuda(LaunchPdl(kern, dim3((unsigned)(units * p.Cluster)), dim3(PD_THREADS), smem, s, args, p.Cluster), "tsa_paged_decode launch");
     }
     unsigned ctas = 0;
     rc = LaunchPagedRanges(p, kv, D, e4m3, (long long)(p.C.Pos || longest < window ? longest : window) / PD_RANGE_TILE + 2, &ctas, s);
