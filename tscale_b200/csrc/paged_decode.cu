@@ -479,6 +479,20 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
             }
         }
     }
+    // this CTA's keys' weights so far are on their way while the sums are joined
+    constexpr int OWN_KEYS = 4 * PD_MIN_TILES * PD_TILE / PD_THREADS; // of a thread at most
+    constexpr size_t NOWHERE = ~(size_t)0;
+    const int keyFirst = max(keyBeg, segBeg * PD_TILE);
+    size_t slotAt[OWN_KEYS];
+    float before[OWN_KEYS];
+    if (track) {
+#pragma unroll
+        for (int i = 0; i < OWN_KEYS; ++i) {
+            const int key = keyFirst + i * PD_THREADS + tid, page = key < keyEnd ? table[key >> c.PageShift] : -1;
+            slotAt[i] = (unsigned)page < (unsigned)c.PageCount ? PlaneSlot(c, page, head) + (key & ((1 << c.PageShift) - 1)) : NOWHERE;
+            before[i] = slotAt[i] != NOWHERE ? c.Weight[slotAt[i]] : 0.0f;
+        }
+    }
     __syncthreads();
     // the CTA's sums: in the place of its first warp's
     for (int x = tid; x < rows * D; x += PD_THREADS) {
@@ -560,16 +574,17 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
         StoreFromFloat(p.Out.Row(seq), (firstHead + r) * D + d, p.OutDtype, a);
     }
     if (track) {
-        // the weights of this CTA's keys (one unit per key head: nobody else adds to them)
-        for (int key = max(keyBeg, segBeg * PD_TILE) + tid; key < keyEnd; key += PD_THREADS) {
-            const int page = table[key >> c.PageShift];
-            if ((unsigned)page < (unsigned)c.PageCount) {
+        // one unit per key head: nobody else adds to them
+#pragma unroll
+        for (int i = 0; i < OWN_KEYS; ++i) {
+            const int key = keyFirst + i * PD_THREADS + tid;
+            if (slotAt[i] != NOWHERE) {
                 float w = 0;
 #pragma unroll 4
                 for (int r = 0; r < rows; ++r) {
                     w += Exp2(logits[r * p.LogitRow + key - segBeg * PD_TILE] - lseOf[r]);
                 }
-                c.Weight[PlaneSlot(c, page, head) + (key & ((1 << c.PageShift) - 1))] += w;
+                c.Weight[slotAt[i]] = before[i] + w;
             }
         }
     }
