@@ -203,9 +203,8 @@ struct TSelectParams {
 
 constexpr int SEL_BINS = 2048;            // 11, 11 and 10 bits of the order
 constexpr int SEL_MAX_CLUSTER = 8;
-constexpr int SEL_SLOTS = 4096;           // slots of a CTA where there are CTAs enough
 constexpr int SEL_LIST = 2048;            // orders of a CTA that are counted from a list instead of from all
-constexpr int SEL_THREADS = 256;          // of a CTA; 1024 where there are too few CTAs
+constexpr int SEL_THREADS = 256;          // of a CTA; or 1024
 constexpr int SEL_PER_SM = 4;
 constexpr int SEL_AHEAD = 2;              // steps of a warp whose loads are under way together
 constexpr int SEL_MAX_SLICE = 44 * 1024;  // slots whose orders fit shared memory
@@ -683,6 +682,41 @@ __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM :
     }
 }
 
+// CTAs of a key head, their threads and slots: the least of what the forms are expected to take, in ns.  Measured on 8 .. 1024 key heads of
+// 256 .. 64000 slots: a CTA alone on its SM takes 4.6 us and 1.28 ns a slot with 256 threads, 5.8 us and 0.65 ns with 1024 (1.6 ns where it
+// reads the weights again in every pass); the exchange inside a cluster 4.5 us; CTAs that share an SM slow each other by 30 to 50 %.  What comes
+// of it, in us: 8 heads of 1000 slots 5.8 with 256 threads, 6.7 with 1024; of 4000 10.0 and 7.9; of 64000 in 8 CTAs 20.9 and 16.6, in one 100;
+// 256 heads of 4000 13.5 and 15.4.
+struct TSelectForm {
+    int Threads, Cluster, Slice;
+};
+static TSelectForm SelectForm(long long units, int longest, int sms)
+{
+    TSelectForm best = {};
+    long long least = 0;
+    for (int threads = SEL_THREADS; threads <= 1024; threads += 1024 - SEL_THREADS) {
+        for (int cluster = 1; cluster <= SEL_MAX_CLUSTER; cluster *= 2) {
+            const bool many = threads > SEL_THREADS;
+            const int warps = cluster * threads / 32, slice = ((longest + warps - 1) / warps + 127) / 128 * 128 * (threads / 32);
+            const bool cached = slice <= SEL_MAX_SLICE;
+            const int room = 227 * 1024 / (int)((many ? sizeof(TSelectShared<32>) : sizeof(TSelectShared<SEL_THREADS / 32>)) + 1024 + (cached ? 4 * slice : 0));
+            const int perSm = many ? 1 : room < SEL_PER_SM ? room : SEL_PER_SM;
+            if (!many && !cached) {
+                continue; // 1024 threads read twice as fast
+            }
+            const long long ctas = units * cluster, onSm = (ctas + sms - 1) / sms, waves = (onSm + perSm - 1) / perSm;
+            const long long alone = (many ? 5800 + (cached ? 65ll : 160ll) * slice / 100 : 4600 + 128ll * slice / 100) + (cluster > 1 ? 4500 : 0);
+            const long long sharing = onSm < perSm ? onSm : perSm;
+            const long long time = waves * alone * (sharing == 1 ? 10 : 12 + sharing / 2) / 10;
+            if (least == 0 || time < least) {
+                least = time;
+                best = {threads, cluster, slice};
+            }
+        }
+    }
+    return best;
+}
+
 // ---- the moves ---------------------------------------------------------------------------------------------------------------
 struct TMoveParams {
     TPages C;
@@ -865,16 +899,10 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_evict_select(con
     if (rc != TSA_OK) {
         return rc;
     }
-    // CTAs of SEL_SLOTS slots while all of them are resident at once (four to an SM); where even then a CTA has twice as many, of twice the
-    // threads
-    p.Cluster = 1;
-    while (p.Cluster < SEL_MAX_CLUSTER && longest > SEL_SLOTS * p.Cluster && 2ll * p.Cluster * kv->kv_heads * nSeq <= 4ll * sms) {
-        p.Cluster *= 2;
-    }
-    const bool many = longest > 2 * SEL_SLOTS * p.Cluster;
-    const int threads = many ? 1024 : SEL_THREADS, warps = p.Cluster * threads / 32;
-    const int slice = ((longest + warps - 1) / warps + 127) / 128 * 128 * (threads / 32);
-    const bool cached = slice <= SEL_MAX_SLICE;
+    const TSelectForm form = SelectForm((long long)kv->kv_heads * nSeq, longest, sms);
+    p.Cluster = form.Cluster;
+    const int threads = form.Threads, slice = form.Slice;
+    const bool many = threads > SEL_THREADS, cached = slice <= SEL_MAX_SLICE;
     const void *kern = many ? (cached ? (const void *)PagedSelectKernel<1024, true> : (const void *)PagedSelectKernel<1024, false>)
                             : (const void *)PagedSelectKernel<SEL_THREADS, true>;
     const size_t smem = cached ? (size_t)slice * sizeof(unsigned) : 0;
