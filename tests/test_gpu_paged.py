@@ -492,7 +492,8 @@ def _select_ref(w, pos, n, newest, keep, recent):
     ([0, 1, 31, 32, 33, 500, 1500], 3, 16, 32, 4, True, "smooth"), ([700, 100], 2, 64, 99, 0, True, "few"), ([5000, 4097], 1, 256, 4096, 4096, True, "zeros"),
     ([3000, 900], 2, 32, 1000, 7, False, "special"), ([2049], 1, 16, 1, 1, True, "smooth"), ([1025, 1024], 1, 32, 1024, 100, True, "few"),
     ([40000], 1, 64, 5000, 64, True, "few"), ([30000, 100000], 1, 16, 70001, 0, True, "few"),
-    ([60000] + [10] * 24, 12, 64, 5000, 8, True, "few")])  # the last: more than a CTA's shared memory holds
+    ([60000] + [10] * 24, 12, 64, 5000, 8, True, "few"),
+    ([400000, 260001], 1, 256, 9000, 100, True, "smooth"), ([750000], 1, 256, 5000, 8, False, "few")])  # the last: more than sixteen CTAs' shared memory holds
 def test_select(lens, kvh, page, keep, recent, positions, values):
     from tscale_b200 import ops
     c = Cache(12, lens, kvh, 64, page, "i8", torch.float16, True)

@@ -202,7 +202,7 @@ struct TSelectParams {
 };
 
 constexpr int SEL_BINS = 2048;            // 11, 11 and 10 bits of the order
-constexpr int SEL_MAX_CLUSTER = 8;
+constexpr int SEL_MAX_CLUSTER = 16, SEL_PORTABLE_CLUSTER = 8, SEL_MOST_SIXTEENS = 6; // six clusters of sixteen CTAs of 1024 threads fit at once
 constexpr int SEL_LIST = 2048;            // orders of a CTA that are counted from a list instead of from all
 constexpr int SEL_THREADS = 256;          // of a CTA; or 1024
 constexpr int SEL_PER_SM = 4;
@@ -684,9 +684,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM :
 
 // CTAs of a key head, their threads and slots: the least of what the forms are expected to take, in ns.  Measured on 8 .. 1024 key heads of
 // 256 .. 64000 slots: a CTA alone on its SM takes 4.6 us and 1.28 ns a slot with 256 threads, 5.8 us and 0.65 ns with 1024 (1.6 ns where it
-// reads the weights again in every pass); the exchange inside a cluster 4.5 us; CTAs that share an SM slow each other by 30 to 50 %.  What comes
-// of it, in us: 8 heads of 1000 slots 5.8 with 256 threads, 6.7 with 1024; of 4000 10.0 and 7.9; of 64000 in 8 CTAs 20.9 and 16.6, in one 100;
-// 256 heads of 4000 13.5 and 15.4.
+// reads the weights again in every pass); the exchange inside a cluster 4.5 us, of sixteen CTAs 10; CTAs that share an SM slow each other by 30 to
+// 50 %.  What comes of it, in us: 8 heads of 1000 slots 5.8 with 256 threads, 6.7 with 1024; of 4000 10.0 and 7.9; of 64000 in 8 CTAs 20.9 and 16.6,
+// in one 100; of 400000 in 8 CTAs 94, in 16 63, of 6 heads 34; 256 heads of 4000 13.5 and 15.4.
 struct TSelectForm {
     int Threads, Cluster, Slice;
 };
@@ -701,11 +701,13 @@ static TSelectForm SelectForm(long long units, int longest, int sms)
             const bool cached = slice <= SEL_MAX_SLICE;
             const int room = 227 * 1024 / (int)((many ? sizeof(TSelectShared<32>) : sizeof(TSelectShared<SEL_THREADS / 32>)) + 1024 + (cached ? 4 * slice : 0));
             const int perSm = many ? 1 : room < SEL_PER_SM ? room : SEL_PER_SM;
-            if (!many && !cached) {
+            const bool sixteen = cluster > SEL_PORTABLE_CLUSTER;
+            if (!many && (!cached || sixteen)) {
                 continue; // 1024 threads read twice as fast
             }
-            const long long ctas = units * cluster, onSm = (ctas + sms - 1) / sms, waves = (onSm + perSm - 1) / perSm;
-            const long long alone = (many ? 5800 + (cached ? 65ll : 160ll) * slice / 100 : 4600 + 128ll * slice / 100) + (cluster > 1 ? 4500 : 0);
+            const long long ctas = units * cluster, onSm = (ctas + sms - 1) / sms;
+            const long long waves = sixteen ? (units + SEL_MOST_SIXTEENS - 1) / SEL_MOST_SIXTEENS : (onSm + perSm - 1) / perSm;
+            const long long alone = (many ? 5800 + (cached ? 65ll : 160ll) * slice / 100 : 4600 + 128ll * slice / 100) + (sixteen ? 10000 : cluster > 1 ? 4500 : 0);
             const long long sharing = onSm < perSm ? onSm : perSm;
             const long long time = waves * alone * (sharing == 1 ? 10 : 12 + sharing / 2) / 10;
             if (least == 0 || time < least) {
@@ -908,6 +910,12 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_evict_select(con
     const size_t smem = cached ? (size_t)slice * sizeof(unsigned) : 0;
     if (smem > 8 * 1024) { // beyond 48 KB with the counts.  The same limit in every call: another thread's may come between this and the launch
         rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_SLICE * sizeof(unsigned)), "cudaFuncSetAttribute");
+        if (rc != TSA_OK) {
+            return rc;
+        }
+    }
+    if (p.Cluster > SEL_PORTABLE_CLUSTER) {
+        rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "cudaFuncSetAttribute");
         if (rc != TSA_OK) {
             return rc;
         }
