@@ -83,7 +83,9 @@ __device__ __forceinline__ int FindSeq(const int *starts, int nSeq, int row, int
 
 // One warp per row: it finds the row's sequence, slot and page while the row's first 64 pieces of 16 bytes of K and V are on their way, and
 // stores the heads' pieces.  The warps of a CTA have neighbouring rows, which are neighbours in their page, too: scales, positions and
-// weights are stored by all of them, a sector of eight rows at a time.
+// weights are stored by all of them, a sector of eight rows at a time (one row at a time, by the row's warp: 42.9 us below instead of 38).
+// Bound by the bytes, read once and written once: 9 prompts of 700 .. 4096 rows of 16 heads x 128 with positions and weights, 250 MB, in 38 to 40 us;
+// 64 single tokens in 4, which is the host's call.
 template <int D, bool SCALE_F16>
 __global__ void __launch_bounds__(APP_WARPS * 32) PagedAppendKernel(const TAppendParams p)
 {
@@ -333,8 +335,13 @@ __device__ __forceinline__ void FindBin(const unsigned *hist, int lane, int take
 // One cluster of CTAs per (sequence, key head); CTA `rank` has the slots [rank * slice, (rank + 1) * slice), each warp a contiguous run of
 // them, four to a lane.  The keep-th largest order is found in three digits: counts of the digit among the orders that agree in the digits
 // before (shared memory; a cluster's CTAs add theirs to the first one's, which finds the digit), then the sum from the top.  The orders that agree with
-// the first digit are few: they go into a list, which the other digits are counted from.  Ranks in slot order are ballots on top of the
+// the first digit are few: they go into a list, which the last digit is counted from.  Ranks in slot order are ballots on top of the
 // sums of the warps and CTAs before.  CACHED: the orders stay in shared memory after they are read once.
+//
+// Not bound by its bytes, 8 per slot read once, but by what depends on one another: page, weight, count, sum, three times over, and the ranks at
+// the end.  40 x 8 key heads of 2000 .. 6144 slots: 15 us (2 at the copy's bandwidth); 2 x 4 of 100000 .. 131072: 21 us (1.4).  Of 28 K clocks of the
+// former the loads take 6.6 K, each search of a digit 1.1 K, the pass over the second digit 4.8 K, the ranks 2.6 K and the moves 7 K; of the latter each
+// digit's exchange 3 to 5 K.  Loads of three, four or six steps ahead instead of two, or three CTAs to an SM instead of four, change nothing.
 template <int THREADS, bool CACHED>
 __global__ void __launch_bounds__(THREADS, THREADS == SEL_THREADS ? SEL_PER_SM : 1) PagedSelectKernel(const TSelectParams p)
 {
@@ -731,8 +738,9 @@ struct TMoveParams {
 constexpr int MOV_WARPS = 4;
 
 // A warp takes 32 moves: each lane looks up the pages of one and carries its scales, position and weight; then 2 D / 16 lanes at a time
-// carry a row of K and V, MOV_AHEAD rows of a lane on their way together.  Sources and destinations of a head are different slots (sources
-// lie behind the budget), so no order is needed.
+// carry a row of K and V, MOV_AHEAD rows of a lane on their way together (46.9 us below with one).  Sources and destinations of a head are
+// different slots (sources lie behind the budget), so no order is needed.  Bound by rows of 64 or 128 bytes and by planes of which a sector of 32 bytes is
+// moved for 2 or 4: 40 caches of 8 heads x 128 cut from up to 6144 to 2048 slots, 180 MB without that, in 39 us.
 constexpr int MOV_AHEAD = 8;
 template <int D, int SCALE_BYTES>
 __global__ void __launch_bounds__(MOV_WARPS * 32) PagedMoveKernel(const TMoveParams p)
