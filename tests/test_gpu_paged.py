@@ -440,21 +440,23 @@ def test_append(kv, scale, kvh, d, page, counts, track, lead):
     assert all(_same(a, b) for a, b in zip((c.k.view(torch.int8), c.v.view(torch.int8), c.ks, c.vs, c.pos, c.weight), want))
 
 
-def test_append_many_sequences():
+@pytest.mark.parametrize("n,kvh,d", [(1500, 1, 64), (2500, 3, 64), (2500, 5, 128)])
+def test_append_many_sequences(n, kvh, d):
     from tscale_b200 import ops
-    counts = [(s * 7919) % 5 for s in range(1500)]
-    c = Cache(10, [n + s % 3 for s, n in enumerate(counts)], 1, 64, 16, "i8", torch.float16, False)
+    counts = [(s * 7919) % 5 for s in range(n)]
+    c = Cache(10, [m + s % 3 for s, m in enumerate(counts)], kvh, d, 16, "i8", torch.float16, False)
     gen, rows = _gen(10), sum(counts)
-    k, v = _codes((rows, 64), "i8", gen), _codes((rows, 64), "i8", gen)
-    ks, vs = torch.rand((1, rows), generator=gen, device=DEV), torch.rand((1, rows), generator=gen, device=DEV)
+    k, v = _codes((rows, kvh * d), "i8", gen), _codes((rows, kvh * d), "i8", gen)
+    ks, vs = torch.rand((kvh, rows), generator=gen, device=DEV), torch.rand((kvh, rows), generator=gen, device=DEV)
     starts = np.concatenate([[0], np.cumsum(counts)])
-    slot = np.concatenate([np.arange(c.lens[s] - n, c.lens[s]) for s, n in enumerate(counts)])
-    seq = np.repeat(np.arange(1500), counts)
+    slot = np.concatenate([np.arange(c.lens[s] - m, c.lens[s]) for s, m in enumerate(counts)])
+    seq = np.repeat(np.arange(n), counts)
     ops.paged_append(c.kv, c.table, c.ctx, k, ks, v, vs, torch.tensor(starts, dtype=torch.int32, device=DEV))
     page = c.table[torch.from_numpy(seq).to(DEV), torch.from_numpy(slot // 16).to(DEV)].long()
     off = torch.from_numpy(slot % 16).to(DEV)
-    assert torch.equal(c.k[page, 0, off], k) and torch.equal(c.v[page, 0, off], v)
-    assert torch.equal(c.ks[page, 0, off], ks[0].half()) and torch.equal(c.vs[page, 0, off], vs[0].half())
+    for h in range(kvh):
+        assert torch.equal(c.k[page, h, off], k[:, h * d:(h + 1) * d]) and torch.equal(c.v[page, h, off], v[:, h * d:(h + 1) * d])
+        assert torch.equal(c.ks[page, h, off], ks[h].half()) and torch.equal(c.vs[page, h, off], vs[h].half())
 
 
 def test_append_places_that_do_not_exist():

@@ -55,46 +55,50 @@ struct TAppendParams {
     TPages C;
     const int *CtxLens, *Tokens, *RowStarts;
     int NSeq, Rows;
+    int LaneShift; // log2 of the lanes of a row
     P2D<char> KNew, VNew;
     P2D<float> KScaleNew, VScaleNew;
     int *Status;
 };
 
-constexpr int APP_WARPS = 8;
+constexpr int APP_AHEAD = 4, APP_MANY_ROWS = 4096;
+constexpr int APP_WARPS = 8, APP_MAX_ROWS = 64; // of a CTA: four lanes to a row at least
 
-// the sequence whose rows [starts[s], starts[s + 1]) hold `row`: the last s with starts[s] <= row, -1 if row is in front of all or behind the
-// last.  A warp narrows the range by 33 per step (sequences without rows have equal starts and are stepped over).
-__device__ __forceinline__ int FindSeq(const int *starts, int nSeq, int row, int lane)
+// The sequence whose rows [starts[s], starts[s + 1]) hold `row`: the last s with starts[s] <= row, -1 if row is in front of all or behind the
+// last.  The 2^shift lanes of a row narrow the range by one more than they are per step (sequences without rows have equal starts and are
+// stepped over); the warp's rows take as many steps as the one that needs most.
+__device__ __forceinline__ int FindSeq(const int *starts, int nSeq, int row, int lane, int shift)
 {
-    if (starts[0] > row || starts[nSeq] <= row) {
-        return -1;
-    }
-    int lo = 0, hi = nSeq; // starts[lo] <= row < starts[hi]
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32;
-        const int at = min(lo + (lane + 1) * step, hi);
+    const int lanes = 1 << shift, l = lane & (lanes - 1);
+    const unsigned mine = (0xffffffffu >> (32 - lanes)) << (lane - l);
+    const bool in = starts[0] <= row && starts[nSeq] > row;
+    int lo = 0, hi = in ? nSeq : 1; // starts[lo] <= row < starts[hi]
+    while (__any_sync(0xffffffffu, hi - lo > 1)) {
+        const int step = (hi - lo + lanes - 1) >> shift;
+        const int at = min(lo + (l + 1) * step, hi);
         const bool below = at < hi && starts[at] <= row;
-        const int cnt = __popc(__ballot_sync(0xffffffffu, below));
+        const int cnt = __popc(__ballot_sync(0xffffffffu, below) & mine);
         hi = min(hi, lo + (cnt + 1) * step);
         lo += cnt * step;
     }
-    return lo;
+    return in ? lo : -1;
 }
 
-// One warp per row: it finds the row's sequence, slot and page while the row's first 64 pieces of 16 bytes of K and V are on their way, and
-// stores the heads' pieces.  The warps of a CTA have neighbouring rows, which are neighbours in their page, too: scales, positions and
+// A warp, or a part of one, per row: it finds the row's sequence, slot and page while the row's first 8 pieces of 16 bytes a lane are on their way,
+// and stores the heads' pieces.  The warps of a CTA have neighbouring rows, which are neighbours in their page, too: scales, positions and
 // weights are stored by all of them, a sector of eight rows at a time (one row at a time, by the row's warp: 42.9 us below instead of 38).
 // Bound by the bytes, read once and written once: 9 prompts of 700 .. 4096 rows of 16 heads x 128 with positions and weights, 250 MB, in 38 to 40 us;
 // 64 single tokens in 4, which is the host's call.
 template <int D, bool SCALE_F16>
 __global__ void __launch_bounds__(APP_WARPS * 32) PagedAppendKernel(const TAppendParams p)
 {
-    constexpr int LPH = D / 16, AHEAD = 4;
+    constexpr int LPH = D / 16, AHEAD = APP_AHEAD;
     constexpr size_t NOWHERE = ~(size_t)0;
-    __shared__ size_t firstOf[APP_WARPS]; // where the rows' tokens are in the planes of head 0
-    __shared__ int posOf[APP_WARPS];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int row0 = blockIdx.x * APP_WARPS, row = row0 + warp;
+    __shared__ size_t firstOf[APP_MAX_ROWS]; // where the rows' tokens are in the planes of head 0
+    __shared__ int posOf[APP_MAX_ROWS];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int lanes = 1 << p.LaneShift, l = lane & (lanes - 1), rows = APP_WARPS * 32 >> p.LaneShift; // of the CTA
+    const int row0 = blockIdx.x * rows, mine = tid >> p.LaneShift, row = row0 + mine;
     PdlTrigger();
     PdlWait();
     const TPages &c = p.C;
@@ -104,61 +108,61 @@ __global__ void __launch_bounds__(APP_WARPS * 32) PagedAppendKernel(const TAppen
     auto load = [&](int i) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            if (i + j * 32 < pieces) {
-                a[j] = __ldg(ks + i + j * 32);
-                b[j] = __ldg(vs + i + j * 32);
+            if (i + j * lanes < pieces) {
+                a[j] = __ldg(ks + i + j * lanes);
+                b[j] = __ldg(vs + i + j * lanes);
             }
         }
     };
     // the scales that this thread will store: of head h0 and row r of the CTA
-    const int r = tid % APP_WARPS, h0 = tid / APP_WARPS;
+    const int r = tid & (rows - 1), h0 = tid / rows;
     float sk = 0, sv = 0;
     if (h0 < c.KvHeads && row0 + r < p.Rows) {
         sk = p.KScaleNew.Row(h0)[row0 + r];
         sv = p.VScaleNew.Row(h0)[row0 + r];
     }
-    size_t first = NOWHERE;
     if (row < p.Rows) {
         ks = reinterpret_cast<const int4 *>(p.KNew.Row(row));
         vs = reinterpret_cast<const int4 *>(p.VNew.Row(row));
-        load(lane);
-        int seq = row, back = 1;
-        if (p.RowStarts) {
-            seq = FindSeq(p.RowStarts, p.NSeq, row, lane);
-            back = seq < 0 ? 0 : p.RowStarts[seq + 1] - row;
+    }
+    load(l);
+    int seq = row < p.Rows ? row : -1, back = 1;
+    if (p.RowStarts) {
+        seq = FindSeq(p.RowStarts, p.NSeq, row, lane, p.LaneShift);
+        back = seq < 0 ? 0 : p.RowStarts[seq + 1] - row;
+    }
+    size_t first = NOWHERE;
+    if (seq >= 0 && row < p.Rows) {
+        const int len = p.CtxLens[seq], slot = len - back, col = slot >> c.PageShift;
+        int page = -1;
+        if (slot >= 0 && col < c.TableCols) {
+            page = c.Table.Row(seq)[col];
         }
-        if (seq >= 0) {
-            const int len = p.CtxLens[seq], slot = len - back, col = slot >> c.PageShift;
-            int page = -1;
-            if (slot >= 0 && col < c.TableCols) {
-                page = c.Table.Row(seq)[col];
+        if ((unsigned)page < (unsigned)c.PageCount) {
+            first = PlaneSlot(c, page, 0) + (slot & ((1 << c.PageShift) - 1)); // the next head's is a page of slots further
+            if (l == 0) {
+                posOf[mine] = (p.Tokens ? p.Tokens[seq] : len) - back;
             }
-            if ((unsigned)page < (unsigned)c.PageCount) {
-                first = PlaneSlot(c, page, 0) + (slot & ((1 << c.PageShift) - 1)); // the next head's is a page of slots further
-                if (lane == 0) {
-                    posOf[warp] = (p.Tokens ? p.Tokens[seq] : len) - back;
-                }
-            } else if (lane == 0 && p.Status) {
-                atomicOr(p.Status, kDevBadSpan); // no such place: nothing is stored
-            }
+        } else if (l == 0 && p.Status) {
+            atomicOr(p.Status, kDevBadSpan); // no such place: nothing is stored
         }
     }
-    if (lane == 0) {
-        firstOf[warp] = first;
+    if (l == 0) {
+        firstOf[mine] = first;
     }
     if (first != NOWHERE) {
-        for (int i = lane;;) {
+        for (int i = l;;) {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
-                const int x = i + j * 32;
+                const int x = i + j * lanes;
                 if (x < pieces) {
                     const size_t at = (first + ((size_t)(x / LPH) << c.PageShift)) * LPH + x % LPH;
                     reinterpret_cast<int4 *>(c.K)[at] = a[j];
                     reinterpret_cast<int4 *>(c.V)[at] = b[j];
                 }
             }
-            i += 32 * AHEAD;
-            if (i - lane >= pieces) {
+            i += lanes * AHEAD;
+            if (i - l >= pieces) {
                 break;
             }
             load(i);
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(APP_WARPS * 32) PagedAppendKernel(const TAppen
     if (firstOf[r] == NOWHERE) {
         return;
     }
-    for (int h = h0; h < c.KvHeads; h += 32) {
+    for (int h = h0; h < c.KvHeads; h += APP_WARPS * 32 / rows) {
         const size_t at = firstOf[r] + ((size_t)h << c.PageShift);
         if (h > h0) {
             sk = p.KScaleNew.Row(h)[row0 + r];
@@ -862,11 +866,19 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_append(const tsa
     p.KScaleNew = P2D<float>(kScaleNew);
     p.VScaleNew = P2D<float>(vScaleNew);
     p.Status = statusWord;
+    // Lanes of a row: a piece for each, or, where there are rows enough to fill the device, as many as they can have under way.  Measured, in us, by
+    // pieces a lane (1, 4; a whole warp for each row): 200000 rows of one head x 128 26.8, 19.4 (81), of 4 x 64 51.7, 35.6 (84), of 12 x 64 118, 101 (118);
+    // 64 rows of 4 x 64 2.5, 3.6 (2.4), 1024 of them 3.3, 4.1 (3.1)
+    const int most = rows < APP_MANY_ROWS ? 1 : APP_AHEAD;
+    p.LaneShift = 2;
+    while (p.LaneShift < 5 && (most << p.LaneShift) < rowBytes / 16) {
+        ++p.LaneShift;
+    }
     const bool f16 = cfg->scale_dtype == TSA_F16;
     const void *kern = cfg->head_dim == 128 ? (f16 ? (const void *)PagedAppendKernel<128, true> : (const void *)PagedAppendKernel<128, false>)
                                             : (f16 ? (const void *)PagedAppendKernel<64, true> : (const void *)PagedAppendKernel<64, false>);
     void *args[] = {&p};
-    return CheckCuda(LaunchPdl(kern, dim3((rows + APP_WARPS - 1) / APP_WARPS), dim3(APP_WARPS * 32), 0, (cudaStream_t)stream, args), "tsa_paged_append launch");
+    return CheckCuda(LaunchPdl(kern, dim3((rows - 1) / (APP_WARPS * 32 >> p.LaneShift) + 1), dim3(APP_WARPS * 32), 0, (cudaStream_t)stream, args), "tsa_paged_append launch");
 }
 
 extern "C" __attribute__((visibility("default"))) int tsa_paged_evict_select(const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens,
