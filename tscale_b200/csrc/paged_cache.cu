@@ -208,7 +208,7 @@ struct TSelectParams {
 };
 
 constexpr int SEL_BINS = 2048;            // 11, 11 and 10 bits of the order
-constexpr int SEL_MAX_CLUSTER = 16, SEL_PORTABLE_CLUSTER = 8, SEL_MOST_SIXTEENS = 6; // six clusters of sixteen CTAs of 1024 threads fit at once
+constexpr int SEL_MAX_CLUSTER = 16, SEL_PORTABLE_CLUSTER = 8;
 constexpr int SEL_LIST = 2048;            // orders of a CTA that are counted from a list instead of from all
 constexpr int SEL_THREADS = 256;          // of a CTA; or 1024
 constexpr int SEL_PER_SM = 4;
@@ -716,8 +716,10 @@ static TSelectForm SelectForm(long long units, int longest, int sms)
             if (!many && (!cached || sixteen)) {
                 continue; // 1024 threads read twice as fast
             }
-            const long long ctas = units * cluster, onSm = (ctas + sms - 1) / sms;
-            const long long waves = sixteen ? (units + SEL_MOST_SIXTEENS - 1) / SEL_MOST_SIXTEENS : (onSm + perSm - 1) / perSm;
+            // SMs that clusters find place on: all of a cluster have to be in one part of the chip.  Of CTAs that have an SM each, 74 clusters of two ran at
+            // once, 33 of four (35 in two waves), 15 of eight and 6 of sixteen
+            const int used = cluster <= 2 ? sms : cluster == 4 ? 132 : cluster == 8 ? (many ? 120 : 128) : 96;
+            const long long ctas = units * cluster, onSm = (ctas + used - 1) / used, waves = (onSm + perSm - 1) / perSm;
             const long long alone = (many ? 5800 + (cached ? 65ll : 160ll) * slice / 100 : 4600 + 128ll * slice / 100) + (sixteen ? 10000 : cluster > 1 ? 4500 : 0);
             const long long sharing = onSm < perSm ? onSm : perSm;
             const long long time = waves * alone * (sharing == 1 ? 10 : 12 + sharing / 2) / 10;
