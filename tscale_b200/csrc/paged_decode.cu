@@ -594,18 +594,18 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     }
 }
 
-// where a sequence's tiles begin in the row of all, and how long the ranges are; by one warp
+// where a sequence's places begin in the row of all, and how long the ranges are; by one warp
 __device__ __forceinline__ void SeqStart(const TPagedDecodeParams &p, int seq, int lane, unsigned ctas, unsigned *start, unsigned *per)
 {
-    int before = 0, all = 0;
+    unsigned before = 0, all = 0;
     for (int s = lane; s < p.NSeq; s += 32) {
-        const int n = SeqTiles<PD_RANGE_TILE>(p, s).Count;
+        const unsigned n = UnitPlaces(SeqTiles<PD_RANGE_TILE>(p, s));
         before += s < seq ? n : 0;
         all += n;
     }
     const int units = p.C.KvHeads * p.HeadChunks;
-    *start = (unsigned)__reduce_add_sync(0xffffffffu, before) * units;
-    *per = RangeTiles((unsigned)__reduce_add_sync(0xffffffffu, all) * units, ctas);
+    *start = __reduce_add_sync(0xffffffffu, before) * units;
+    *per = RangePlaces(__reduce_add_sync(0xffffffffu, all) * units, ctas);
 }
 
 // records base + i * stride, i = first, first + step, ..: their sums of 4 dimensions (column 4 sub) and of the weights, relative to m
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(FIN_THREADS) PagedJoinKernel(const TPagedDecod
         SeqStart(p, seg.Seq, lane, ctas, &start, &per);
         seg.Keys = SeqTiles<PD_RANGE_TILE>(p, seg.Seq);
         if (seg.Keys.Count > 0) {
-            start += (unsigned)seg.Unit * seg.Keys.Count;
+            start += (unsigned)seg.Unit * UnitPlaces(seg.Keys) + PD_UNIT_TILES;
             first = start / per;
             chunks = (start + seg.Keys.Count - 1) / per - first + 1;
             chunks = chunks > 1 ? chunks : 0;
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(FIN_THREADS) PagedJoinKernel(const TPagedDecod
         TRangeWalk walk;
         if (walk.Begin(p, lane, blockIdx.x, ctas, false)) {
             seg = walk.Segment(p);
-            start = walk.SeqBase + (unsigned)seg.Unit * seg.Keys.Count;
+            start = walk.SeqBase + (unsigned)seg.Unit * UnitPlaces(seg.Keys) + PD_UNIT_TILES;
             if (walk.At > start && walk.At - walk.Per <= start) {
                 first = blockIdx.x - 1;
                 chunks = (start + seg.Keys.Count - 1) / walk.Per - first + 1;
@@ -898,7 +898,7 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     const bool track = kv->weight != nullptr;
     const long long room = TableTokens(p.C);
     const int longest = room < maxCtx ? (int)room : maxCtx;
-    const long long units = (long long)nSeq * kv->kv_heads * p.HeadChunks, tilesMax = (long long)longest / PD_TILE + 2;
+    const long long units = (long long)nSeq * kv->kv_heads * p.HeadChunks, tilesMax = (long long)longest / PD_TILE + 8;
     TSA_REQUIRE(units * tilesMax < (1ll << 31), "tsa_paged_decode: %d sequences of %d tokens with %d query heads are too much for one call", nSeq, longest, headCount);
     const TPagedForm form = PagedForm(D, nSeq, kv->kv_heads, headCount, maxCtx, window, kv->pos != nullptr, track);
     TSA_REQUIRE(form.Bytes == 0 || (workspace && workspaceBytes >= form.Bytes), "tsa_paged_decode: workspace of %zu bytes needed, %zu given", form.Bytes, workspaceBytes);
