@@ -57,7 +57,7 @@ struct TTcMisc {
     uint32_t TmemBase;
     int Abort;
     int Fresh[2];                // the product with these weights starts a new sum
-    alignas(16) float Mult[PD_ROWS];        // query scale times the logits' factor
+    alignas(16) float Mult[2][PD_ROWS];     // query scale times the logits' factor, of this unit and the next
     alignas(16) float Ref[PD_ROWS];
     float Red[PT_SOFT_WARPS][PD_ROWS];
     alignas(16) float Factor[PD_ROWS];
@@ -349,10 +349,7 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
             const TSegment seg = walk.Segment(p);
             for (int tile = seg.TileBeg; tile < seg.TileEnd && ok; ++tile, ++count) {
                 const bool newUnit = tile == seg.TileBeg;
-                if (newUnit && count > 0) {
-                    weigh(count - 1); // the arithmetic threads end the unit before they bring the next one's queries
-                }
-                if (newUnit && ok) {
+                if (newUnit) { // there before the last weights of the unit before
                     wait(&misc.QReady, segments & 1, kDevTimeoutMma);
                 }
                 const int stage = count % STAGES, buf = count & 1;
@@ -376,7 +373,7 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
                     MmaCommit(&misc.SReady[buf]);
                 }
                 __syncwarp();
-                if (!newUnit) {
+                if (count > 0) {
                     weigh(count - 1);
                 }
             }
@@ -399,27 +396,45 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
         // dimension of this thread's lane of the result: all 128 lanes, or 16 of each warp's
         const int dim = D == 128 ? tid : warp * 16 + lane;
         const bool hasDim = D == 128 || lane < 16;
-        int count = 0;
+        int count = 0, segments = 0;
         bool dead = false;
-        for (bool more = true; more;) {
-            const TSegment seg = walk.Segment(p);
-            const int head = seg.Unit / p.HeadChunks, chunk = seg.Unit % p.HeadChunks;
-            const int firstHead = head * p.Group + chunk * PD_ROWS, rows = min(p.Group - chunk * PD_ROWS, PD_ROWS);
-            // the queries as a K-major tile with the swizzle of the keys (all products with the unit's before are done)
-            if (tid < PD_ROWS * D / 16) {
-                const int r = tid / (D / 16), piece = tid % (D / 16);
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (r < rows) {
-                    x = *reinterpret_cast<const uint4 *>(p.Q.Row(seg.Seq) + (firstHead + r) * D + piece * 16);
-                }
-                *reinterpret_cast<uint4 *>(qTile + r * D + (D == 128 ? piece ^ (r & 7) : piece ^ (r >> 1 & 3)) * 16) = x;
+        // a unit's queries, a piece of 16 bytes to a thread, and their scales
+        uint4 query = make_uint4(0, 0, 0, 0);
+        float mult = 0;
+        auto loadQueries = [&](const TSegment &s) {
+            const int chunk = s.Unit % p.HeadChunks, firstHead = s.Unit / p.HeadChunks * p.Group + chunk * PD_ROWS, rows = min(p.Group - chunk * PD_ROWS, PD_ROWS);
+            const int r = tid / (D / 16), piece = tid % (D / 16);
+            query = make_uint4(0, 0, 0, 0);
+            if (r < rows) {
+                query = *reinterpret_cast<const uint4 *>(p.Q.Row(s.Seq) + (firstHead + r) * D + piece * 16);
+            }
+            mult = p.QVecScale;
+            if (tid < rows && p.QScale.Valid()) {
+                mult = p.QScale.Row(s.Seq)[firstHead + tid];
+            }
+        };
+        // as a K-major tile with the swizzle of the keys, once all score products with the unit's before are done
+        auto storeQueries = [&](int n) {
+            const int r = tid / (D / 16), piece = tid % (D / 16);
+            if (r < PD_ROWS) {
+                *reinterpret_cast<uint4 *>(qTile + r * D + (D == 128 ? piece ^ (r & 7) : piece ^ (r >> 1 & 3)) * 16) = query;
             }
             if (tid < PD_ROWS) {
-                misc.Mult[tid] = tid < rows ? p.DotScale * (p.QScale.Valid() ? p.QScale.Row(seg.Seq)[firstHead + tid] : p.QVecScale) : 0.0f;
-                misc.Ref[tid] = PD_NO_REF;
+                misc.Mult[n & 1][tid] = p.DotScale * mult;
             }
             FenceProxyAsync();
             MbarArrive(&misc.QReady);
+        };
+        loadQueries(walk.Segment(p));
+        storeQueries(0);
+        for (bool more = true; more; ++segments) {
+            const TSegment seg = walk.Segment(p);
+            const int head = seg.Unit / p.HeadChunks, chunk = seg.Unit % p.HeadChunks;
+            const int firstHead = head * p.Group + chunk * PD_ROWS, rows = min(p.Group - chunk * PD_ROWS, PD_ROWS);
+            more = walk.Next(p, seg);
+            if (tid < PD_ROWS) {
+                misc.Ref[tid] = PD_NO_REF;
+            }
             float sum[HEADS], acc[HEADS];
 #pragma unroll
             for (int h = 0; h < HEADS; ++h) {
@@ -451,6 +466,10 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
             SoftAny(false); // Mult and Ref are there
             for (int tile = seg.TileBeg; tile < seg.TileEnd; ++tile, ++count) {
                 const int buf = count & 1, stage = count % STAGES, wBuf = count % W_BUFS, key = tile * PT_KEYS + tid;
+                const bool bringNext = more && tile == seg.TileEnd - 1;
+                if (bringNext) {
+                    loadQueries(walk.Segment(p));
+                }
                 if (!dead && !WaitBarA<true>(&misc.KeysFull[stage], (count / STAGES) & 1, abortFlag)) {
                     dead = true;
                     fail(kDevTimeoutMma);
@@ -476,10 +495,13 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
                         z[h] = E4M3 ? __uint_as_float(r[h]) : (float)(int)r[h];
                     }
                 }
+                if (bringNext) {
+                    storeQueries(segments + 1);
+                }
                 bool raise = false;
 #pragma unroll
                 for (int b = 0; b < HB; ++b) {
-                    const float4 m4 = *reinterpret_cast<const float4 *>(&misc.Mult[4 * b]), r4 = *reinterpret_cast<const float4 *>(&misc.Ref[4 * b]);
+                    const float4 m4 = *reinterpret_cast<const float4 *>(&misc.Mult[segments & 1][4 * b]), r4 = *reinterpret_cast<const float4 *>(&misc.Ref[4 * b]);
                     const float mult[4] = {m4.x, m4.y, m4.z, m4.w}, ref[4] = {r4.x, r4.y, r4.z, r4.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -638,7 +660,6 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
                 }
             }
             SoftAny(false); // Red, Ref and Factor have been read
-            more = walk.Next(p, seg);
         }
     }
     TcFenceBefore();
