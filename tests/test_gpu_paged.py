@@ -281,6 +281,36 @@ def test_decode_split_over_long_caches(kv, lens, heads, kvh, d, page, track):
             assert float((c.weight[p, h, o].double() - before[p, h, o].double() - added[0, h]).abs().max()) <= ERR * (heads // kvh) + 2.0 ** -23
 
 
+@pytest.mark.parametrize("kv,scale,d,heads,kvh,page", [("i8", torch.float16, 64, 4, 2, 32), ("e4m3", torch.float32, 128, 6, 1, 128), ("i8", torch.float32, 128, 24, 2, 16),
+                                                       ("e4m3", torch.float16, 64, 40, 2, 256), ("i8", torch.float16, 64, 16, 1, 64)])
+@pytest.mark.parametrize("window,ordered", [(30, False), (0, False), (1000, True), (5000, False), (30, True)])
+def test_decode_windows_of_long_caches_with_positions(kv, scale, d, heads, kvh, page, window, ordered):
+    """Most tiles have no key inside the window, some key heads none at all."""
+    from tscale_b200 import ops
+    lens = [6000, 1, 9000, 0, 140, 20000]
+    c = Cache(21, lens, kvh, d, page, kv, scale, True)
+    for s, n in enumerate(lens):
+        for h in range(kvh):
+            if ordered and n:
+                c.write(c.pos, s, h, c.read(c.pos, s, h).sort().values.to(torch.int32))
+    p, o = c.place(2)
+    c.pos[p, kvh - 1, o] = 0  # nothing in the window of the last key head
+    q, qs = _query(21, len(lens), heads, d, kv)
+    before = c.weight.clone()
+    want, added = _decode_ref(c, q, qs, heads, window, 0.0)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, 0.0, max_ctx=max(lens), tokens=c.tokens, status=status)
+    assert int(status) == 0
+    _check_out(got, want, c)
+    for (s, h), w in added.items():
+        p, o = c.place(s)
+        assert float((c.weight[p, h, o].double() - before[p, h, o].double() - w).abs().max()) <= ERR * (heads // kvh) + 2.0 ** -23
+    # a page outside the pool is reported from a tile that nobody needs, too
+    c.table[5, 3] = 1 << 20
+    ops.paged_decode(c.kv, c.table, c.ctx, q, qs, 30, 0.0, max_ctx=max(lens), tokens=c.tokens, status=status)
+    assert int(status) != 0
+
+
 def test_decode_no_key_inside_the_window_and_no_query_scale():
     from tscale_b200 import ops
     c = Cache(3, [300, 40], 2, 64, 32, "e4m3", torch.float16, True)
