@@ -347,15 +347,16 @@ size_t tsa_att_decode_static_capacity_bytes(void);
  * A pool of page_count pages is shared by all sequences; a page holds page_size tokens of all key heads, head by head:
  *   k, v                8-bit [page_count][kv_heads][page_size][D];   k_scale, v_scale  scale_dtype [page_count][kv_heads][page_size]
  *   pos    int32 [page_count][kv_heads][page_size]  positions of the tokens, for caches that are evicted from (NULL: a token's
- *                                                   position is its slot)
+ *                                                   position is its slot); those of a key head's tokens are different numbers
  *   weight f32   [page_count][kv_heads][page_size]  attention weights that the tokens have gathered (NULL: not kept)
  * all contiguous, in device memory, 16-byte aligned.  Slot t of sequence s is slot t % page_size of page pageTable[s][t / page_size]
  * (int32 [nSeq][maxPages], device memory; entries behind a sequence's last page are not read).  ctxLens[s] (device) is the number of
  * slots that the sequence fills; tokens[s] (device; NULL without pos) the number of tokens that it has seen, so that its newest token
  * has position tokens[s] - 1 (ctxLens[s] - 1 without pos).  A row of the table has room for 2^30 tokens at most.  Sequences may share
  * pages (of a common beginning, say) where no call writes to them: append and evict_move write, and so does decode to weight.
- * A page number outside the pool, or a length beyond the table's or the caller's bound, sets a bit of the status word; the rows
- * concerned are not stored, attended, chosen or moved, and nothing outside the buffers is touched. */
+ * A page number outside the pool, a length beyond the table's or the caller's bound, or more tokens of a key head inside a short window
+ * than it has positions sets a bit of the status word; the rows concerned are not stored, attended, chosen or moved, and nothing outside
+ * the buffers is touched. */
 typedef struct {
     void *k;
     void *v;

@@ -311,6 +311,24 @@ def test_decode_windows_of_long_caches_with_positions(kv, scale, d, heads, kvh, 
     assert int(status) != 0
 
 
+def test_decode_positions_that_repeat():
+    """More keys inside the window than it has positions: reported, and the others of the batch are right."""
+    from tscale_b200 import ops
+    c = Cache(22, [5000, 3000], 1, 64, 64, "i8", torch.float16, True)
+    q, qs = _query(22, 2, 4, 64, "i8")
+    want, added = _decode_ref(c, q, qs, 4, 100, 0.0)
+    p, o = c.place(0)
+    c.pos[p, 0, o] = int(c.tokens[0]) - 5
+    before = c.weight.clone()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, 100, 0.0, max_ctx=5000, tokens=c.tokens, status=status)
+    assert int(status) != 0
+    c.lens[0] = 0
+    _check_out(got[1:], want[1:], c)
+    p, o = c.place(1)
+    assert float((c.weight[p, 0, o].double() - before[p, 0, o].double() - added[1, 0]).abs().max()) <= 4 * ERR + 2.0 ** -23
+
+
 def test_decode_no_key_inside_the_window_and_no_query_scale():
     from tscale_b200 import ops
     c = Cache(3, [300, 40], 2, 64, 32, "e4m3", torch.float16, True)

@@ -76,7 +76,8 @@ def test_types_that_are_refused(kw):
     (_decode, dict(kv=_kv(pos=None)), b"go together"), (_decode, dict(q=NULL), b"null"), (_decode, dict(q=abi.Ptr2D(FAKE, 256, 255, 3)), b"extents"),
     (_decode, dict(q=abi.Ptr2D(FAKE, 264, 256, 3)), b"aligned"), (_decode, dict(out=abi.Ptr2D(FAKE, 1024, 256, 2)), b"extents"),
     (_decode, dict(out=abi.Ptr2D(FAKE + 4, 1024, 256, 3)), b"aligned"), (_decode, dict(qs=_plane(3, 3)), b"qScale"), (_decode, dict(qs=_plane(4, 3, stride=18)), b"qScale"),
-    (_decode, dict(ws=None, max_ctx=20000), b"workspace"), (_decode, dict(ws=None, max_ctx=20000, kv=_kv(weight=None)), b"workspace"), (_decode, dict(ws_bytes=100, max_ctx=20000), b"workspace"), (_decode, dict(ws=FAKE + 8), b"workspace"),
+    (_decode, dict(ws=None, max_ctx=20000, window=5000), b"workspace"), (_decode, dict(ws=None, max_ctx=20000, window=5000, kv=_kv(weight=None)), b"workspace"),
+    (_decode, dict(ws_bytes=100, max_ctx=20000, window=5000), b"workspace"), (_decode, dict(ws=FAKE + 8), b"workspace"),
     (_decode, dict(n=60000, table=_plane(1 << 24, 60000), max_ctx=1 << 29, q=abi.Ptr2D(FAKE, 256, 256, 60000), out=abi.Ptr2D(FAKE, 1024, 256, 60000)), b"too much"),
     (_select, dict(kv=_kv(weight=None)), b"weights"), (_select, dict(keep=0), b"keep"), (_select, dict(recent=51), b"keep"), (_select, dict(recent=-1), b"keep"),
     (_select, dict(tokens=None), b"go together"), (_select, dict(cap=49), b"room for 50"), (_select, dict(cap=0, max_ctx=40), b"room for 1"),
@@ -97,6 +98,7 @@ def test_workspace_sizes():
         ctypes.byref(_cfg()), ctypes.byref(_kv(**kw)), n, heads, ctx, window)
     assert need(3, 4, 200) == need(3, 4, 200, weight=None) == 0  # a cluster per key head
     assert need(3, 4, 20000) - need(3, 4, 20000, weight=None) == 256 + 3 * 4 * 20000 * 4 and need(3, 4, 20000, weight=None) > 0
+    assert need(3, 4, 20000, 64) == 0 and need(3, 4, 20000, 1500) > 0  # a short window: its keys are listed in shared memory
     assert need(3, 4, 20000, 64, pos=None, weight=None) == 0 and need(300, 4, 20000, 64, pos=None, weight=None) == 0
     assert need(0, 4, 200) == 0 and need(3, 1, 200) == 0 and need(3, 4, -1) == 0 and need(3, 4, 200, -1) == 0
 

@@ -7,7 +7,8 @@
 // The stream of the cache bounds it: 2 D bytes of codes and two scales per key and key head, each read once; for short caches the latency
 // of what depends on one another does.  Two forms:
 //   clusters (here): a cluster of up to 8 CTAs has a unit (the up to 16 query heads that share a key head of a sequence) and joins its sums
-//     through distributed shared memory: one kernel, for caches of up to 4096 slots while all clusters are resident at once.
+//     through distributed shared memory: one kernel, for caches of up to 4096 slots while all clusters are resident at once, and for windows of
+//     up to 1024 positions of longer caches with positions, whose keys it lists first.
 //   ranges (paged_decode_sm100.cu): all keys of all units, in a row, are cut into equal ranges, one for each CTA that can be resident; a
 //     unit that a range border cuts leaves partial sums, which a second kernel joins in the order of the ranges.
 // No atomics in either: the same bits every time.  Measured: 12 heads x 64 of one sequence of 1000 slots 5.3 us (the host's call takes as long); 64
@@ -32,6 +33,7 @@ constexpr int PD_THREADS = PD_WARPS * 32;
 constexpr int PD_TILE = 16;              // keys of a warp's tile
 constexpr int PD_MIN_TILES = 8;          // of a CTA: two tiles per warp
 constexpr int PD_MAX_CLUSTER = 8;
+constexpr int PD_MAX_LIST = 1024;        // keys that a CTA lists
 
 __device__ __forceinline__ uint4 LoadStream(const void *p)
 {
@@ -98,6 +100,12 @@ template <>
 struct TScales<true> {
     uint2 X;
     __device__ __forceinline__ void Load(const char *p, size_t at) { X = LoadStream8(p + at * 2); }
+    __device__ __forceinline__ void Gather(const char *p, const size_t (&at)[4])
+    {
+        const unsigned short *s = reinterpret_cast<const unsigned short *>(p);
+        const unsigned a = s[at[0]], b = s[at[1]], c = s[at[2]], d = s[at[3]];
+        X = make_uint2(a | b << 16, c | d << 16);
+    }
     __device__ __forceinline__ float Get(int i) const
     {
         const uint32_t w = i < 2 ? X.x : X.y;
@@ -108,6 +116,11 @@ template <>
 struct TScales<false> {
     uint4 X;
     __device__ __forceinline__ void Load(const char *p, size_t at) { X = LoadStream(p + at * 4); }
+    __device__ __forceinline__ void Gather(const char *p, const size_t (&at)[4])
+    {
+        const unsigned *s = reinterpret_cast<const unsigned *>(p);
+        X = make_uint4(s[at[0]], s[at[1]], s[at[2]], s[at[3]]);
+    }
     __device__ __forceinline__ float Get(int i) const { return __uint_as_float(i == 0 ? X.x : i == 1 ? X.y : i == 2 ? X.z : X.w); }
 };
 
@@ -121,7 +134,9 @@ __device__ __forceinline__ float ClusterLoad(const float *mine, int rank)
 // One cluster of p.Cluster CTAs per unit.  WIDE: more than eight query heads share a key head (otherwise rows 8 .. 15 of the scores are
 // unused, and half the sums).  A warp works on U tiles of 16 keys at a time, 4 KB of K and V, and holds the loads of its next ones in
 // registers meanwhile.
-template <int D, bool E4M3, bool SCALE_F16, bool WIDE>
+// SPARSE: of a cache with positions, whose tokens may be in any order, and a window much shorter than it.  The CTA looks at the positions of its
+// slots first and lists those inside the window; its tiles are then 16 of the list each, gathered row by row.
+template <int D, bool E4M3, bool SCALE_F16, bool WIDE, bool SPARSE>
 __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(const TPagedDecodeParams p)
 {
     constexpr int U = 128 / D, STEP = PD_WARPS * U;
@@ -131,6 +146,10 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     constexpr int ROWS = 8 * HALVES;
     typedef typename std::conditional<D == 128, uint4, uint2>::type TPiece; // D / 8 dimensions of a key
     extern __shared__ __align__(16) float logits[]; // of this CTA's keys, [rows][p.LogitRow]
+    // SPARSE, behind the logits: where the listed keys are in the planes, and how far from the query's position
+    size_t *const listAt = reinterpret_cast<size_t *>(logits + (p.C.Weight ? p.Rows * p.LogitRow : 0));
+    int *const listFar = reinterpret_cast<int *>(listAt + p.ListCap);
+    __shared__ int listOf[PD_WARPS];
     __shared__ __align__(16) float accOf[PD_WARPS][ROWS][D + 4]; // [.][.][16 j + 2 g + b] for dimension D / 8 g + 2 j + b: no two lanes of a store meet in a bank
     __shared__ float refOf[PD_WARPS][ROWS], sumOf[PD_WARPS][ROWS], ctaRef[ROWS], ctaSum[ROWS], lseOf[ROWS], factorOf[ROWS][PD_MAX_CLUSTER];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -145,15 +164,96 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     }
     const TSeqKeys keys = SeqTiles<PD_TILE>(p, seq);
     const int per = (keys.Count + ctas - 1) / ctas;
-    const int segBeg = keys.First + min(rank * per, keys.Count), segEnd = min(segBeg + per, keys.First + keys.Count);
+    int segBeg = keys.First + min(rank * per, keys.Count), segEnd = min(segBeg + per, keys.First + keys.Count);
     const int cur = (p.Tokens ? p.Tokens[seq] : p.CtxLens[seq]) - 1;
     const int *table = c.Table.Row(seq);
     const int tileShift = c.PageShift - 4, tileMask = (1 << tileShift) - 1;
     // keys of this CTA; a key at distance cur - position is attended if (unsigned)(distance - nearest) < spread
-    const int keyBeg = keys.Beg, keyEnd = min(keys.End, segEnd * PD_TILE);
+    int keyBeg = keys.Beg, keyEnd = min(keys.End, segEnd * PD_TILE);
     const int nearest = p.Window > 0 ? 1 : 0;
     const unsigned spread = p.Window > 0 ? p.Window : 1;
     const bool track = c.Weight != nullptr;
+    bool badPage = false;
+    if (SPARSE) {
+        // each warp has a contiguous part of the CTA's slots; it counts, then it lists them
+        const int slots = ((keyEnd - segBeg * PD_TILE + PD_WARPS - 1) / PD_WARPS + 3) & ~3;
+        const int beg = segBeg * PD_TILE + warp * slots, end = min(beg + slots, keyEnd);
+        int at = 0;
+        auto scan = [&](bool write) {
+            constexpr int AHEAD = 4;
+            for (int s0 = beg; s0 < end; s0 += 128 * AHEAD) {
+                int page[AHEAD];
+                int4 pos[AHEAD];
+                size_t where[AHEAD];
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int s = s0 + 128 * j + 4 * lane;
+                    page[j] = s < end ? table[s >> c.PageShift] : 0;
+                    badPage |= (unsigned)page[j] >= (unsigned)c.PageCount;
+                }
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int s = s0 + 128 * j + 4 * lane;
+                    where[j] = PlaneSlot(c, (unsigned)page[j] < (unsigned)c.PageCount ? page[j] : 0, head) + (s & ((1 << c.PageShift) - 1));
+                    pos[j] = *reinterpret_cast<const int4 *>(c.Pos + where[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int s = s0 + 128 * j + 4 * lane, far[4] = {cur - pos[j].x, cur - pos[j].y, cur - pos[j].z, cur - pos[j].w};
+                    unsigned in = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        in |= (unsigned)(s + i < end && (unsigned)page[j] < (unsigned)c.PageCount && (unsigned)(far[i] - nearest) < spread) << i;
+                    }
+                    if (!__any_sync(0xffffffffu, in)) {
+                        continue;
+                    }
+                    int before = __popc(in);
+                    const int mine = before;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int v = __shfl_up_sync(0xffffffffu, before, o);
+                        before += lane >= o ? v : 0;
+                    }
+                    if (write) {
+                        int to = at + before - mine;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (in >> i & 1) {
+                                if (to < p.ListCap) {
+                                    listAt[to] = where[j] + i;
+                                    listFar[to] = far[i];
+                                }
+                                ++to;
+                            }
+                        }
+                    }
+                    at += __shfl_sync(0xffffffffu, before, 31);
+                }
+            }
+        };
+        scan(false);
+        if (lane == 0) {
+            listOf[warp] = at;
+        }
+        __syncthreads();
+        at = 0;
+        keyEnd = 0;
+#pragma unroll
+        for (int w = 0; w < PD_WARPS; ++w) {
+            at += w < warp ? listOf[w] : 0;
+            keyEnd += listOf[w];
+        }
+        scan(true);
+        __syncthreads();
+        // from here on, keys are places of the list.  It has room for a key at each position of the window; where positions repeat, for no more
+        if (keyEnd > p.ListCap && tid == 0 && p.Status) {
+            atomicOr(p.Status, kDevBadSpan);
+        }
+        keyEnd = min(keyEnd, p.ListCap);
+        keyBeg = segBeg = 0;
+        segEnd = (keyEnd + PD_TILE - 1) / PD_TILE;
+    }
 
     // the query heads of this lane's rows, in the dimensions' order of the fragments
     uint32_t qa[KS][4];
@@ -203,10 +303,11 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     int4 ps[U];
     const int keyRow = 4 * (g >> 1) + (g & 1); // of score block 0
     const size_t kLane = (size_t)keyRow * D + t * 16, vLane = (size_t)(4 * t) * D + g * (D / 8);
-    auto pageOf = [&](int tile) { return tile < segEnd ? table[tile >> tileShift] : -1; };
+    auto pageOf = [&](int tile) { return SPARSE ? 0 : tile < segEnd ? table[tile >> tileShift] : -1; };
+    auto listed = [&](size_t i) { return listAt[min((int)i, keyEnd - 1)]; };
     // the slots of a tile; a tile that there is not, or whose page is outside the pool, reads page 0 and is masked
     auto slotOf = [&](int tile, int page) {
-        return PlaneSlot(c, (unsigned)page < (unsigned)c.PageCount ? page : 0, head) + ((tile & tileMask) << 4);
+        return SPARSE ? (size_t)tile * PD_TILE : PlaneSlot(c, (unsigned)page < (unsigned)c.PageCount ? page : 0, head) + ((tile & tileMask) << 4);
     };
     auto loadK = [&](const size_t (&slot)[U]) {
 #pragma unroll
@@ -214,10 +315,17 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
             const uint8_t *src = c.K + slot[u] * D + kLane;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
+                const uint8_t *row = SPARSE ? c.K + listed(slot[u] + keyRow + 2 * n) * D + t * 16 : src + 2 * n * D;
 #pragma unroll
                 for (int i = 0; i < D / 64; ++i) {
-                    kr[u][n][i] = LoadStream(src + 2 * n * D + i * 64);
+                    kr[u][n][i] = LoadStream(row + i * 64);
                 }
+            }
+            if (SPARSE) {
+                const size_t at[4] = {listed(slot[u] + 4 * t), listed(slot[u] + 4 * t + 1), listed(slot[u] + 4 * t + 2), listed(slot[u] + 4 * t + 3)};
+                ks[u].Gather(c.KScale, at);
+                vs[u].Gather(c.VScale, at);
+                continue;
             }
             ks[u].Load(c.KScale, slot[u] + 4 * t);
             vs[u].Load(c.VScale, slot[u] + 4 * t); // with K: the weights need it before V
@@ -232,12 +340,11 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
             const uint8_t *src = c.V + slot[u] * D + vLane;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                LoadStream(src + i * D, &vr[u][i]);
+                LoadStream(SPARSE ? c.V + listed(slot[u] + 4 * t + i) * D + g * (D / 8) : src + i * D, &vr[u][i]);
             }
         }
     };
 
-    bool badPage = false;
     int tile = segBeg + warp * U;
     if (tile < segEnd) {
         size_t slot[U];
@@ -311,7 +418,12 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
             for (int u = 0; u < U; ++u) {
                 const int key0 = (tile + u) * PD_TILE + 4 * t;
                 int far[4] = {cur - key0, cur - key0 - 1, cur - key0 - 2, cur - key0 - 3};
-                if (c.Pos) {
+                if (SPARSE) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        far[i] = listFar[min(key0 + i, keyEnd - 1)];
+                    }
+                } else if (c.Pos) {
                     far[0] = cur - ps[u].x;
                     far[1] = cur - ps[u].y;
                     far[2] = cur - ps[u].z;
@@ -336,7 +448,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
                     }
                 }
                 // a tile in the middle of the range of a cache without positions has no masked key
-                if (!okNow[u] || c.Pos || (tile + u) * PD_TILE < keyBeg || (tile + u + 1) * PD_TILE > keyEnd) {
+                if (!okNow[u] || (!SPARSE && c.Pos) || (tile + u) * PD_TILE < keyBeg || (tile + u + 1) * PD_TILE > keyEnd) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const bool valid = okNow[u] && key0 + i >= keyBeg && key0 + i < keyEnd && (unsigned)(far[i] - nearest) < spread;
@@ -481,7 +593,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
         }
     }
     // this CTA's keys' weights so far are on their way while the sums are joined
-    constexpr int OWN_KEYS = 4 * PD_MIN_TILES * PD_TILE / PD_THREADS; // of a thread at most
+    constexpr int OWN_KEYS = (SPARSE ? PD_MAX_LIST : 4 * PD_MIN_TILES * PD_TILE) / PD_THREADS; // of a thread at most
     constexpr size_t NOWHERE = ~(size_t)0;
     const int keyFirst = max(keyBeg, segBeg * PD_TILE);
     size_t slotAt[OWN_KEYS];
@@ -489,8 +601,13 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     if (track) {
 #pragma unroll
         for (int i = 0; i < OWN_KEYS; ++i) {
-            const int key = keyFirst + i * PD_THREADS + tid, page = key < keyEnd ? table[key >> c.PageShift] : -1;
-            slotAt[i] = (unsigned)page < (unsigned)c.PageCount ? PlaneSlot(c, page, head) + (key & ((1 << c.PageShift) - 1)) : NOWHERE;
+            const int key = keyFirst + i * PD_THREADS + tid;
+            if (SPARSE) {
+                slotAt[i] = key < keyEnd ? listAt[key] : NOWHERE;
+            } else {
+                const int page = key < keyEnd ? table[key >> c.PageShift] : -1;
+                slotAt[i] = (unsigned)page < (unsigned)c.PageCount ? PlaneSlot(c, page, head) + (key & ((1 << c.PageShift) - 1)) : NOWHERE;
+            }
             before[i] = slotAt[i] != NOWHERE ? c.Weight[slotAt[i]] : 0.0f;
         }
     }
@@ -809,7 +926,9 @@ struct TPagedForm {
     // parts of the workspace, in this order
     size_t Partial, Lse, Logits, Bytes;
     int LogitRow;
+    int ListCap; // keys that a CTA lists; 0: none
 };
+constexpr int PD_SPARSE_MIN = 1024, PD_SPARSE_SLOTS = 512;
 constexpr int B200_SMS = 148, PD_MAX_CLUSTER_SMS = 128;
 static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, int maxCtx, int window, bool positions, bool track)
 {
@@ -832,8 +951,27 @@ static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, i
     if (!(inTime || one) || (track && chunks > 1)) {
         w.Cluster = 0;
     }
+    // A window much shorter than a cache with positions: its keys may be anywhere, so all slots have to be looked at, but only by their positions, and
+    // the window's rows alone are read.  Pays from half the cache on against the ranges, a quarter against clusters that read all, which are short of
+    // bytes to save and have no list to wait for.  Measured with and without, in us, units of four int8 heads x 128, windows 64 / 1000:
+    //   units x slots   4 x 8192         32 x 4096         128 x 8192        512 x 3000         1024 x 8192      32 x 400000
+    //   with            7.2 / 9.5        7.9 / 10.9        9.7 / 17.0        12.4 / 36.7        34 / 92          47 / 60
+    //   without         11.5 / 11.6      14.0 / 14.0       42.8 / 42.6       62.6 / 62.5        278 / 278        401 / 401
+    // 512 slots to a CTA (1024: 4 units of 1500 slots, window 250, 9.2 instead of 8.1), as far as eight CTAs go.
+    w.ListCap = 0;
+    const int listMax = window == 0 ? 1 : window;
+    if (positions && listMax <= PD_MAX_LIST && maxCtx > PD_SPARSE_MIN && maxCtx / listMax >= (w.Cluster ? 4 : 2) && !(track && chunks > 1)) {
+        w.Cluster = 1;
+        while (w.Cluster < PD_MAX_CLUSTER && maxCtx > PD_SPARSE_SLOTS * w.Cluster) {
+            w.Cluster *= 2;
+        }
+        while (w.Cluster > 1 && !resident()) {
+            w.Cluster /= 2;
+        }
+        w.ListCap = (listMax + PD_TILE - 1) / PD_TILE * PD_TILE;
+    }
     // clusters: of a CTA, an odd number of tiles, so that the rows of a store lie in different banks
-    w.LogitRow = w.Cluster ? (int)((tilesMax + w.Cluster - 1) / w.Cluster | 1) * PD_TILE
+    w.LogitRow = w.ListCap ? (w.ListCap / PD_TILE | 1) * PD_TILE : w.Cluster ? (int)((tilesMax + w.Cluster - 1) / w.Cluster | 1) * PD_TILE
                            : (int)((maxCtx < 0x7ffffff0 ? (long long)maxCtx + PD_TILE - 1 : 0x7ffffff0ll) / PD_TILE * PD_TILE);
     w.Partial = 0;
     w.Lse = w.Logits = w.Bytes = 0; // a cluster has all it needs in shared memory
@@ -845,11 +983,16 @@ static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, i
     return w;
 }
 
-template <int D, bool E4M3>
-static const void *PickCluster(bool f16, bool wide)
+template <int D, bool E4M3, bool SPARSE>
+static const void *PickWidth(bool f16, bool wide)
 {
-    return f16 ? (wide ? (const void *)PagedClusterKernel<D, E4M3, true, true> : (const void *)PagedClusterKernel<D, E4M3, true, false>)
-               : (wide ? (const void *)PagedClusterKernel<D, E4M3, false, true> : (const void *)PagedClusterKernel<D, E4M3, false, false>);
+    return f16 ? (wide ? (const void *)PagedClusterKernel<D, E4M3, true, true, SPARSE> : (const void *)PagedClusterKernel<D, E4M3, true, false, SPARSE>)
+               : (wide ? (const void *)PagedClusterKernel<D, E4M3, false, true, SPARSE> : (const void *)PagedClusterKernel<D, E4M3, false, false, SPARSE>);
+}
+template <int D, bool E4M3>
+static const void *PickCluster(bool f16, bool wide, bool sparse)
+{
+    return sparse ? PickWidth<D, E4M3, true>(f16, wide) : PickWidth<D, E4M3, false>(f16, wide);
 }
 
 } // namespace tsa
@@ -920,6 +1063,7 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     p.Lse = track ? (float *)((char *)workspace + form.Lse) : nullptr;
     p.Logits = track ? (float *)((char *)workspace + form.Logits) : nullptr;
     p.LogitRow = form.LogitRow;
+    p.ListCap = form.ListCap;
     p.Status = statusWord;
     p.Cluster = form.Cluster;
     const bool e4m3 = cfg->kv_dtype == TSA_E4M3, f16 = cfg->scale_dtype == TSA_F16;
@@ -927,12 +1071,14 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     cudaStream_t s = (cudaStream_t)stream;
     if (form.Cluster) {
         const bool wide = p.Group > 8;
-        const void *kern = D == 128 ? (e4m3 ? PickCluster<128, true>(f16, wide) : PickCluster<128, false>(f16, wide))
-                                    : (e4m3 ? PickCluster<64, true>(f16, wide) : PickCluster<64, false>(f16, wide));
-        const size_t smem = track ? p.Rows * form.LogitRow * sizeof(float) : 0;
-        if (smem > 0 && wide) { // beyond 48 KB with what the kernel has anyway; the same limit in every call
-            rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PD_ROWS * (4 * PD_MIN_TILES + 1) * PD_TILE * sizeof(float)),
-                "cudaFuncSetAttribute");
+        const bool sparse = form.ListCap > 0;
+        const void *kern = D == 128 ? (e4m3 ? PickCluster<128, true>(f16, wide, sparse) : PickCluster<128, false>(f16, wide, sparse))
+                                    : (e4m3 ? PickCluster<64, true>(f16, wide, sparse) : PickCluster<64, false>(f16, wide, sparse));
+        const size_t smem = (track ? p.Rows * form.LogitRow * sizeof(float) : 0) + form.ListCap * (sizeof(size_t) + sizeof(int));
+        if (smem > 0 && (wide || sparse)) { // beyond 48 KB with what the kernel has anyway; the same limit in every call
+            const int most = sparse ? PD_MAX_LIST : 4 * PD_MIN_TILES * PD_TILE;
+            rc = CheckCuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                (wide ? PD_ROWS : 8) * (most + PD_TILE) * (int)sizeof(float) + (sparse ? PD_MAX_LIST * (int)(sizeof(size_t) + sizeof(int)) : 0)), "cudaFuncSetAttribute");
             if (rc != TSA_OK) {
                 return rc;
             }

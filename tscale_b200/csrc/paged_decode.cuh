@@ -27,6 +27,7 @@ struct TPagedDecodeParams {
     float *Lse;      // [nSeq][heads]: log2 of the weights' sum and the sink (caches that keep weights)
     float *Logits;   // [nSeq][heads][LogitRow]
     int LogitRow;
+    int ListCap;     // keys that a CTA lists, where the kernel does
     int *Status;
 };
 
