@@ -420,9 +420,10 @@ class PagedKVCache:
         self.tokens = self._dev[n_seq * (max_pages + 1):] if evict else None
         self.free = list(range(page_count - 1, -1, -1))
 
-    def _upload(self):
-        host = torch.from_numpy(self._host.copy())
-        self._dev.copy_(host.pin_memory() if self._dev.is_cuda else host, non_blocking=True)
+    def _upload(self, table=True):
+        beg = 0 if table else self.n_seq * self.max_pages
+        host = torch.from_numpy(self._host[beg:].copy())
+        self._dev[beg:].copy_(host.pin_memory() if self._dev.is_cuda else host, non_blocking=True)
 
     def _pages(self, slots):
         return -(-int(slots) // self.page_size)
@@ -433,18 +434,17 @@ class PagedKVCache:
         counts = np.broadcast_to(np.asarray(counts, dtype=np.int64), (self.n_seq,))
         if (counts < 0).any():
             raise abi.TsaError(abi.TSA_BAD_ARG, "PagedKVCache.extend: negative count")
-        after = self.lens + counts
-        need = [self._pages(b) - self._pages(a) for a, b in zip(self.lens, after)]
-        if max(self._pages(n) for n in after) > self.max_pages or sum(need) > len(self.free):
+        have, after = -(-self.lens // self.page_size), -(-(self.lens + counts) // self.page_size)  # pages
+        need = after - have
+        if after.max() > self.max_pages or need.sum() > len(self.free):
             raise abi.TsaError(abi.TSA_BAD_ARG, "PagedKVCache.extend: %d pages needed, %d free; a sequence has at most %d"
-                               % (sum(need), len(self.free), self.max_pages))
-        for s, n in enumerate(need):
-            have = self._pages(self.lens[s])
-            for i in range(n):
-                self._table[s, have + i] = self.free.pop()
+                               % (need.sum(), len(self.free), self.max_pages))
+        for s in np.flatnonzero(need):
+            for i in range(have[s], after[s]):
+                self._table[s, i] = self.free.pop()
         self.lens += counts.astype(np.int32)
         self.seen += counts.astype(np.int32)
-        self._upload()
+        self._upload(need.any())
         if (counts == 1).all():
             return None
         return torch.from_numpy(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)).to(self._dev.device)
