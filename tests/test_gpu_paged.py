@@ -283,8 +283,8 @@ def test_decode_split_over_long_caches(kv, lens, heads, kvh, d, page, track):
 
 @pytest.mark.parametrize("kv,scale,d,heads,kvh,page", [("i8", torch.float16, 64, 4, 2, 32), ("e4m3", torch.float32, 128, 6, 1, 128), ("i8", torch.float32, 128, 24, 2, 16),
                                                        ("e4m3", torch.float16, 64, 40, 2, 256), ("i8", torch.float16, 64, 16, 1, 64)])
-@pytest.mark.parametrize("window,ordered", [(30, False), (0, False), (1000, True), (5000, False), (30, True)])
-def test_decode_windows_of_long_caches_with_positions(kv, scale, d, heads, kvh, page, window, ordered):
+@pytest.mark.parametrize("window,ordered,slope", [(30, False, 0.0), (0, False, 0.0), (1000, True, 0.02), (5000, False, 0.0), (30, True, 0.5), (700, False, 0.01)])
+def test_decode_windows_of_long_caches_with_positions(kv, scale, d, heads, kvh, page, window, ordered, slope):
     """Most tiles have no key inside the window, some key heads none at all."""
     from tscale_b200 import ops
     lens = [6000, 1, 9000, 0, 140, 20000]
@@ -297,11 +297,16 @@ def test_decode_windows_of_long_caches_with_positions(kv, scale, d, heads, kvh, 
     c.pos[p, kvh - 1, o] = 0  # nothing in the window of the last key head
     q, qs = _query(21, len(lens), heads, d, kv)
     before = c.weight.clone()
-    want, added = _decode_ref(c, q, qs, heads, window, 0.0)
+    want, added = _decode_ref(c, q, qs, heads, window, slope)
     status = torch.zeros(1, dtype=torch.int32, device=DEV)
-    got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, 0.0, max_ctx=max(lens), tokens=c.tokens, status=status)
+    got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, slope, max_ctx=max(lens), tokens=c.tokens, status=status)
     assert int(status) == 0
     _check_out(got, want, c)
+    # without the weights, into another type, and the same again
+    plain = c.kv._replace(weight=None)
+    runs = [ops.paged_decode(plain, c.table, c.ctx, q, qs, window, slope, max_ctx=max(lens), tokens=c.tokens, out_dtype=torch.bfloat16) for _ in range(2)]
+    assert torch.equal(*runs)
+    _check_out(runs[0], want, c)
     for (s, h), w in added.items():
         p, o = c.place(s)
         assert float((c.weight[p, h, o].double() - before[p, h, o].double() - w).abs().max()) <= ERR * (heads // kvh) + 2.0 ** -23
