@@ -194,6 +194,14 @@ def test_decode_in_ranges(kv, scale, d, heads, kvh, page, window, slope, out, tr
     _decode_of(MANY, kv, scale, d, heads, kvh, page, window, slope, out, track)
 
 
+@pytest.mark.parametrize("kv,scale,d,heads,kvh,page,window,slope,out,track", [
+    ("i8", torch.float16, 128, 16, 8, 32, WHOLE, 0.0, torch.float32, False), ("e4m3", torch.float32, 64, 96, 8, 16, WHOLE, 0.02, torch.bfloat16, True),
+    ("e4m3", torch.float16, 128, 128, 8, 64, 40, 0.0, torch.float16, False), ("i8", torch.float32, 64, 8, 8, 16, 0, 0.0, torch.float32, True)])
+def test_decode_many_short_sequences(kv, scale, d, heads, kvh, page, window, slope, out, track):
+    """More units of a few tiles than CTAs of four warps would have room for."""
+    _decode_of([0, 1, 2, 15, 16, 17, 97, 111] + [(s * 37) % 60 for s in range(76)], kv, scale, d, heads, kvh, page, window, slope, out, track)
+
+
 @pytest.mark.parametrize("heads,kvh,lens", [(4, 2, [700, 300]), (16, 8, MANY), (12, 1, [513]), (128, 8, MANY)])
 @pytest.mark.parametrize("kv", ["i8", "e4m3"])
 def test_decode_logits_that_rise(heads, kvh, lens, kv):

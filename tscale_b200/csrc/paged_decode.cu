@@ -29,7 +29,7 @@
 namespace tsa {
 
 constexpr int PD_WARPS = 4;
-constexpr int PD_THREADS = PD_WARPS * 32;
+constexpr int PD_ONE_WARP_TILES = 8;     // of a unit that one warp has, at most
 constexpr int PD_TILE = 16;              // keys of a warp's tile
 constexpr int PD_MIN_TILES = 8;          // of a CTA: two tiles per warp
 constexpr int PD_MAX_CLUSTER = 8;
@@ -136,10 +136,12 @@ __device__ __forceinline__ float ClusterLoad(const float *mine, int rank)
 // registers meanwhile.
 // SPARSE: of a cache with positions, whose tokens may be in any order, and a window much shorter than it.  The CTA looks at the positions of its
 // slots first and lists those inside the window; its tiles are then 16 of the list each, gathered row by row.
-template <int D, bool E4M3, bool SCALE_F16, bool WIDE, bool SPARSE>
-__global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(const TPagedDecodeParams p)
+// WARPS: four; one where there are many units of a few tiles.
+template <int D, bool E4M3, bool SCALE_F16, bool WIDE, bool SPARSE, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, (WIDE ? 3 : 4) * (PD_WARPS / WARPS)) PagedClusterKernel(const TPagedDecodeParams p)
 {
-    constexpr int U = 128 / D, STEP = PD_WARPS * U;
+    constexpr int THREADS = WARPS * 32;
+    constexpr int U = 128 / D, STEP = WARPS * U;
     constexpr int MT = D / 16;                      // row blocks of the output, 16 dimensions each
     constexpr int HALVES = WIDE ? 2 : 1;            // blocks of eight query heads
     constexpr int KS = E4M3 ? D / 16 : D / 32;      // steps of the score product
@@ -149,9 +151,9 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     // SPARSE, behind the logits: where the listed keys are in the planes, and how far from the query's position
     size_t *const listAt = reinterpret_cast<size_t *>(logits + (p.C.Weight ? p.Rows * p.LogitRow : 0));
     int *const listFar = reinterpret_cast<int *>(listAt + p.ListCap);
-    __shared__ int listOf[PD_WARPS];
-    __shared__ __align__(16) float accOf[PD_WARPS][ROWS][D + 4]; // [.][.][16 j + 2 g + b] for dimension D / 8 g + 2 j + b: no two lanes of a store meet in a bank
-    __shared__ float refOf[PD_WARPS][ROWS], sumOf[PD_WARPS][ROWS], ctaRef[ROWS], ctaSum[ROWS], lseOf[ROWS], factorOf[ROWS][PD_MAX_CLUSTER];
+    __shared__ int listOf[WARPS];
+    __shared__ __align__(16) float accOf[WARPS][ROWS][D + 4]; // [.][.][16 j + 2 g + b] for dimension D / 8 g + 2 j + b: no two lanes of a store meet in a bank
+    __shared__ float refOf[WARPS][ROWS], sumOf[WARPS][ROWS], ctaRef[ROWS], ctaSum[ROWS], lseOf[ROWS], factorOf[ROWS][PD_MAX_CLUSTER];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const TPages &c = p.C;
     const int unitsPerSeq = c.KvHeads * p.HeadChunks, ctas = p.Cluster, rank = blockIdx.x % ctas, unit = blockIdx.x / ctas;
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     bool badPage = false;
     if (SPARSE) {
         // each warp has a contiguous part of the CTA's slots; it counts, then it lists them
-        const int slots = ((keyEnd - segBeg * PD_TILE + PD_WARPS - 1) / PD_WARPS + 3) & ~3;
+        const int slots = ((keyEnd - segBeg * PD_TILE + WARPS - 1) / WARPS + 3) & ~3;
         const int beg = segBeg * PD_TILE + warp * slots, end = min(beg + slots, keyEnd);
         int at = 0;
         auto scan = [&](bool write) {
@@ -240,7 +242,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
         at = 0;
         keyEnd = 0;
 #pragma unroll
-        for (int w = 0; w < PD_WARPS; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             at += w < warp ? listOf[w] : 0;
             keyEnd += listOf[w];
         }
@@ -593,7 +595,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
         }
     }
     // this CTA's keys' weights so far are on their way while the sums are joined
-    constexpr int OWN_KEYS = (SPARSE ? PD_MAX_LIST : 4 * PD_MIN_TILES * PD_TILE) / PD_THREADS; // of a thread at most
+    constexpr int OWN_KEYS = (SPARSE ? PD_MAX_LIST : WARPS == 1 ? PD_ONE_WARP_TILES * PD_TILE : 4 * PD_MIN_TILES * PD_TILE) / THREADS; // of a thread at most
     constexpr size_t NOWHERE = ~(size_t)0;
     const int keyFirst = max(keyBeg, segBeg * PD_TILE);
     size_t slotAt[OWN_KEYS];
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     if (track) {
 #pragma unroll
         for (int i = 0; i < OWN_KEYS; ++i) {
-            const int key = keyFirst + i * PD_THREADS + tid;
+            const int key = keyFirst + i * THREADS + tid;
             if (SPARSE) {
                 slotAt[i] = key < keyEnd ? listAt[key] : NOWHERE;
             } else {
@@ -613,16 +615,16 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     }
     __syncthreads();
     // the CTA's sums: in the place of its first warp's
-    for (int x = tid; x < rows * D; x += PD_THREADS) {
+    for (int x = tid; x < rows * D; x += THREADS) {
         const int r = x / D, i = x % D;
         float m = refOf[0][r];
 #pragma unroll
-        for (int w = 1; w < PD_WARPS; ++w) {
+        for (int w = 1; w < WARPS; ++w) {
             m = fmaxf(m, refOf[w][r]);
         }
         float a = 0;
 #pragma unroll
-        for (int w = 0; w < PD_WARPS; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             a = fmaf(Exp2(refOf[w][r] - m), accOf[w][r][i], a);
         }
         accOf[0][r][i] = a;
@@ -630,11 +632,11 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     if (tid < rows) {
         float m = refOf[0][tid], s = 0;
 #pragma unroll
-        for (int w = 1; w < PD_WARPS; ++w) {
+        for (int w = 1; w < WARPS; ++w) {
             m = fmaxf(m, refOf[w][tid]);
         }
 #pragma unroll
-        for (int w = 0; w < PD_WARPS; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             s = fmaf(Exp2(refOf[w][tid] - m), sumOf[w][tid], s);
         }
         ctaRef[tid] = m;
@@ -647,9 +649,10 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
     }
     // every CTA of the cluster finishes a part of the result from all their sums: eight threads per row find the factors of the CTAs' sums.
     // The reference is at least -60: the sink, weight 1 at logit 0, then stays in range
-    static_assert(PD_MAX_CLUSTER == 8 && 8 * PD_ROWS <= PD_THREADS, "a thread per row and CTA");
-    {
-        const int r = tid >> 3, i = tid & 7;
+    static_assert(PD_MAX_CLUSTER == 8, "a thread per row and CTA");
+#pragma unroll
+    for (int x = tid; x < 8 * ROWS; x += THREADS) {
+        const int r = x >> 3, i = x & 7;
         const bool in = r < rows && i < ctas;
         const float ref1 = in ? ClusterLoad(&ctaRef[r], i) : PD_NO_REF, sum1 = in ? ClusterLoad(&ctaSum[r], i) : 0.0f;
         float m = fmaxf(ref1, -60.0f);
@@ -672,7 +675,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
         }
     }
     __syncthreads();
-    for (int x = rank * PD_THREADS + tid; x < rows * D; x += ctas * PD_THREADS) {
+    for (int x = rank * THREADS + tid; x < rows * D; x += ctas * THREADS) {
         const int r = x / D, i = x % D;
         const int d = (i >> 1 & 7) * (D / 8) + 2 * (i >> 4) + (i & 1);
         float a = 0;
@@ -695,7 +698,7 @@ __global__ void __launch_bounds__(PD_THREADS, WIDE ? 3 : 4) PagedClusterKernel(c
         // one unit per key head: nobody else adds to them
 #pragma unroll
         for (int i = 0; i < OWN_KEYS; ++i) {
-            const int key = keyFirst + i * PD_THREADS + tid;
+            const int key = keyFirst + i * THREADS + tid;
             if (slotAt[i] != NOWHERE) {
                 float w = 0;
 #pragma unroll 4
@@ -927,6 +930,7 @@ struct TPagedForm {
     size_t Partial, Lse, Logits, Bytes;
     int LogitRow;
     int ListCap; // keys that a CTA lists; 0: none
+    bool OneWarp; // of a CTA
 };
 constexpr int PD_SPARSE_MIN = 1024, PD_SPARSE_SLOTS = 512;
 constexpr int B200_SMS = 148, PD_MAX_CLUSTER_SMS = 128;
@@ -970,6 +974,11 @@ static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, i
         }
         w.ListCap = (listMax + PD_TILE - 1) / PD_TILE * PD_TILE;
     }
+    // A warp per unit where CTAs of four would come in more than one and a half turns, or in more than one for a tile or two of narrow units.
+    // Measured, in us, with one warp and with four, 128 int8 dimensions, two / sixteen query heads a unit: 640 units of 16 slots 5.8, 7.7 / 16.3, 14.9; 1024 of 64
+    // 9.4, 10.0 / 20.6, 23.2; 2048 of 16 7.1, 15.4 / 31, 36; 2048 of 112 14.5, 21.7 / 44.5, 46.2
+    const size_t four = (size_t)B200_SMS * (rows > 8 ? 3 : 4);
+    w.OneWarp = w.Cluster == 1 && w.ListCap == 0 && tilesMax <= PD_ONE_WARP_TILES && (2 * units > 3 * four || (units > four && rows <= 8 && tilesMax <= 3));
     // clusters: of a CTA, an odd number of tiles, so that the rows of a store lie in different banks
     w.LogitRow = w.ListCap ? (w.ListCap / PD_TILE | 1) * PD_TILE : w.Cluster ? (int)((tilesMax + w.Cluster - 1) / w.Cluster | 1) * PD_TILE
                            : (int)((maxCtx < 0x7ffffff0 ? (long long)maxCtx + PD_TILE - 1 : 0x7ffffff0ll) / PD_TILE * PD_TILE);
@@ -983,16 +992,16 @@ static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, i
     return w;
 }
 
-template <int D, bool E4M3, bool SPARSE>
+template <int D, bool E4M3, bool SPARSE, int WARPS>
 static const void *PickWidth(bool f16, bool wide)
 {
-    return f16 ? (wide ? (const void *)PagedClusterKernel<D, E4M3, true, true, SPARSE> : (const void *)PagedClusterKernel<D, E4M3, true, false, SPARSE>)
-               : (wide ? (const void *)PagedClusterKernel<D, E4M3, false, true, SPARSE> : (const void *)PagedClusterKernel<D, E4M3, false, false, SPARSE>);
+    return f16 ? (wide ? (const void *)PagedClusterKernel<D, E4M3, true, true, SPARSE, WARPS> : (const void *)PagedClusterKernel<D, E4M3, true, false, SPARSE, WARPS>)
+               : (wide ? (const void *)PagedClusterKernel<D, E4M3, false, true, SPARSE, WARPS> : (const void *)PagedClusterKernel<D, E4M3, false, false, SPARSE, WARPS>);
 }
 template <int D, bool E4M3>
-static const void *PickCluster(bool f16, bool wide, bool sparse)
+static const void *PickCluster(bool f16, bool wide, bool sparse, bool oneWarp)
 {
-    return sparse ? PickWidth<D, E4M3, true>(f16, wide) : PickWidth<D, E4M3, false>(f16, wide);
+    return sparse ? PickWidth<D, E4M3, true, PD_WARPS>(f16, wide) : oneWarp ? PickWidth<D, E4M3, false, 1>(f16, wide) : PickWidth<D, E4M3, false, PD_WARPS>(f16, wide);
 }
 
 } // namespace tsa
@@ -1072,8 +1081,8 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
     if (form.Cluster) {
         const bool wide = p.Group > 8;
         const bool sparse = form.ListCap > 0;
-        const void *kern = D == 128 ? (e4m3 ? PickCluster<128, true>(f16, wide, sparse) : PickCluster<128, false>(f16, wide, sparse))
-                                    : (e4m3 ? PickCluster<64, true>(f16, wide, sparse) : PickCluster<64, false>(f16, wide, sparse));
+        const void *kern = D == 128 ? (e4m3 ? PickCluster<128, true>(f16, wide, sparse, form.OneWarp) : PickCluster<128, false>(f16, wide, sparse, form.OneWarp))
+                                    : (e4m3 ? PickCluster<64, true>(f16, wide, sparse, form.OneWarp) : PickCluster<64, false>(f16, wide, sparse, form.OneWarp));
         const size_t smem = (track ? p.Rows * form.LogitRow * sizeof(float) : 0) + form.ListCap * (sizeof(size_t) + sizeof(int));
         if (smem > 0 && (wide || sparse)) { // beyond 48 KB with what the kernel has anyway; the same limit in every call
             const int most = sparse ? PD_MAX_LIST : 4 * PD_MIN_TILES * PD_TILE;
@@ -1084,7 +1093,7 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_decode(const tsa
             }
         }
         void *args[] = {&p};
-        return CheckCuda(LaunchPdl(kern, dim3((unsigned)(units * p.Cluster)), dim3(PD_THREADS), smem, s, args, p.Cluster), "tsa_paged_decode launch");
+        return CheckCuda(LaunchPdl(kern, dim3((unsigned)(units * p.Cluster)), dim3(form.OneWarp ? 32 : PD_WARPS * 32), smem, s, args, p.Cluster), "tsa_paged_decode launch");
     }
     unsigned ctas = 0;
     rc = LaunchPagedRanges(p, kv, D, e4m3, (long long)(p.C.Pos || longest < window ? longest : window) / PD_RANGE_TILE + 2, &ctas, s);
