@@ -921,8 +921,10 @@ __global__ void __launch_bounds__(WGT_THREADS) PagedWeightKernel(const TPagedDec
 // makes them so.  Measured, in us, as clusters and as ranges, for units of two int8 heads of 128 dimensions (8 key heads a sequence):
 //   units x slots      8 x 256    64 x 1024   64 x 4000   72 x 1024 (of 4)  128 x 512   256 x 256   256 x 1024 (of 2: left to the ranges)
 //   clusters / ranges  5.5 / 6.6  7.4 / 9.1   14.9 / 15.4     9.0 / 9.7     7.6 / 9.7   7.4 / 8.8   26.9 / 15.8
-// Beyond the resident ones a CTA per unit pays while it has few tiles, 16 (8 for more than eight heads): 1024 units of 128 slots 12.4 / 16.9, of
-// 256 slots 17.0 / 20.9, of 512 slots 31.0 / 32.0, 2048 units of 512 slots 58 / 54.
+// Beyond the resident ones a CTA per unit pays while it has few tiles, 24 of 128 dimensions or 32 of 64:
+//   heads of a unit x D   2 x 128                                    16 x 128                        16 x 64, with weights        4 x 64
+//   units x slots         1024 x 256  1024 x 512  2048 x 512         664 x 384  2048 x 384           664 x 512  2048 x 512        664 x 512  2048 x 512
+//   clusters / ranges     17.0 / 20.9  31.0 / 32.0  58 / 54          27.7 / 32.3  74 / 68            23.4 / 41.5  65 / 103        15.6 / 19.6  40 / 44
 // Units that share a key head's weights leave them to the kernel behind the ranges.
 struct TPagedForm {
     int Cluster; // CTAs of a unit; 0: ranges
@@ -951,7 +953,7 @@ static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, i
     while (w.Cluster > 1 && !resident()) {
         w.Cluster /= 2;
     }
-    const bool inTime = resident() && tilesMax <= 4 * PD_MIN_TILES * w.Cluster, one = w.Cluster == 1 && tilesMax <= PD_MIN_TILES * (rows > 8 ? 1 : 2) + 1;
+    const bool inTime = resident() && tilesMax <= 4 * PD_MIN_TILES * w.Cluster, one = w.Cluster == 1 && tilesMax <= (headDim == 64 ? 4 : 3) * PD_MIN_TILES + 1;
     if (!(inTime || one) || (track && chunks > 1)) {
         w.Cluster = 0;
     }
