@@ -9,8 +9,8 @@
 // what the digits before left over, 16 times larger each (2^-16 of w itself).  The columns cost the tensor cores nothing that shows: 128 x
 // D x 64 per 33 KB of cache.  Each of the 128 arithmetic threads has one key of the tile and the weights of all heads for it.
 //
-// Measured: 64 sequences of 1024 .. 8192 slots, 16 key heads x 128 int8, 1.31 GB: 195 to 205 us, 6.4 to 6.7 TB/s (a plain copy: 6.45; mma.sync with
-// the codes in registers: 213 us); 48 of 500 .. 9000, 8 key heads x 128 e4m3 of four query heads, 0.5 GB: 88 to 94; 2 of 100000 .. 131072, 4 key heads of eight
+// Measured: 64 sequences of 1024 .. 8192 slots, 16 key heads x 128 int8, 1.31 GB: 181 to 205 us, 6.4 to 7.2 TB/s (a plain copy: 6.45; mma.sync with
+// the codes in registers: 213 us); 48 of 500 .. 9000, 8 key heads x 128 e4m3 of four query heads, 0.5 GB: 84 to 94; 2 of 100000 .. 131072, 4 key heads of eight
 // query heads, 0.27 GB: 48.  What short calls lose is the start (lengths, page, first tile: 4 us) and the join; the tensor pipe is at 4 to 6 %, the
 // issue slots at 21 (four heads a unit) to 31 % (eight).
 //
