@@ -34,6 +34,7 @@ constexpr int PD_TILE = 16;              // keys of a warp's tile
 constexpr int PD_MIN_TILES = 8;          // of a CTA: two tiles per warp
 constexpr int PD_MAX_CLUSTER = 8;
 constexpr int PD_MAX_LIST = 1024;        // keys that a CTA lists
+constexpr float PD_EDGE = 8.0f;          // log2 of the largest weight
 
 __device__ __forceinline__ uint4 LoadStream(const void *p)
 {
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(WARPS * 32, (WIDE ? 3 : 4) * (PD_WARPS / WARPS
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    edge[u][i] = ReferenceEdge(vScale[u][i]);
+                    edge[u][i] = ReferenceEdge(vScale[u][i], PD_EDGE);
                 }
             }
             if (more) {
@@ -495,7 +496,7 @@ __global__ void __launch_bounds__(WARPS * 32, (WIDE ? 3 : 4) * (PD_WARPS / WARPS
                     float m = ref[half];
 #pragma unroll
                     for (int i = 0; i < U * 4; ++i) {
-                        m = fmaxf(m, z[i / 4][half][i % 4] - edge[i / 4][i % 4] + 8.0f);
+                        m = fmaxf(m, z[i / 4][half][i % 4] - edge[i / 4][i % 4] + PD_EDGE);
                     }
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));

@@ -43,11 +43,11 @@ __device__ __forceinline__ float Log2(float x)
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// How far the logit of a key may lie above the reference: 2^(z - ref) * vScale stays within 2^8.  Value scales below 2^-80, zero among them,
-// count as that here: weights then stay within 2^88, and the sum of 2^30 of them within float32.
-__device__ __forceinline__ float ReferenceEdge(float vScale)
+// How far the logit of a key may lie above the reference: 2^(z - ref) * vScale stays within 2^headroom.  Value scales below 2^-80, zero among them,
+// count as that here: weights then stay within 2^(80 + headroom), and the sum of 2^30 of them within float32.
+__device__ __forceinline__ float ReferenceEdge(float vScale, float headroom)
 {
-    return 8.0f - fmaxf(Log2(fabsf(vScale)), -80.0f);
+    return headroom - fmaxf(Log2(fabsf(vScale)), -80.0f);
 }
 
 // tiles [First, First + Count) of TILE slots that hold the keys of a sequence; keys are slots [Beg, End) (of a cache with positions, some of

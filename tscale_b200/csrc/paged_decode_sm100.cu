@@ -4,10 +4,10 @@
 // What bounds it is the stream of the cache, so nothing but the copy engine and the tensor cores touches the codes of K and V:
 //   scores  [128 keys][16 heads]      = K tile [128][D] (shared memory, as the pages hold it) * q [16][D]
 //   result  [D][16 columns per 4 heads] += V tile [128][D] read along its rows * weights [128 keys][16 columns per 4 heads]
-// kind::i8 or kind::f8f6f4, accumulators in tensor memory.  A weight w = 2^(z - ref) * vScale, |w| <= 2^8, is four columns of 8 bits that
-// add up to it: for int8 the signed base-256 digits of w * 2^22 (off by 2^-23 of the largest weight), for e4m3 the roundings of w and of
-// what the digits before left over, 16 times larger each (2^-16 of w itself).  The columns cost the tensor cores nothing that shows: 128 x
-// D x 64 per 33 KB of cache.  Each of the 128 arithmetic threads has one key of the tile and the weights of all heads for it.
+// kind::i8 or kind::f8f6f4, accumulators in tensor memory.  A weight w = 2^(z - ref) * vScale, |w| < 2^4, is four columns of 8 bits that
+// add up to it: for int8 the signed base-256 digits of w * 2^27 (off by 2^-28), for e4m3 the roundings of w * 2^4 and of what the digits
+// before left over, 32 times larger each (off by 2^-16 of w, or by 2^-29 if that is more).  The columns cost the tensor cores nothing that
+// shows: 128 x D x 64 per 33 KB of cache.  Each of the 128 arithmetic threads has one key of the tile and the weights of all heads for it.
 //
 // Measured: 64 sequences of 1024 .. 8192 slots, 16 key heads x 128 int8, 1.31 GB: 181 to 205 us, 6.4 to 7.2 TB/s (a plain copy: 6.45; mma.sync with
 // the codes in registers: 213 us); 48 of 500 .. 9000, 8 key heads x 128 e4m3 of four query heads, 0.5 GB: 84 to 94; 2 of 100000 .. 131072, 4 key heads of eight
@@ -17,8 +17,11 @@
 // One CTA: a warp that issues the copies (a box per page, up to 128 slots; tiles ahead of the arithmetic as far as the ring goes, across
 // units), one that issues the products, four for the weights.  Two CTAs per SM: while one of them ends a unit, the other has the memory.
 // Three where a tile is half as large and the weights leave the room (64 dimensions, up to eight heads): 512 key heads of 4000 slots 54 us instead of 61.
-// The reference of a head rises only when a weight would exceed 2^8; the sums so far then leave tensor memory for registers, where they
-// are scaled, and the accumulation starts anew (also before int32 could overflow).  All waits are bounded.
+// What the digits leave out is absolute, so that very many light keys behind a heavy one would be lost beside a reference that only rises (131072
+// keys of 2^-22 of the first: 0.6 % of the sum with int8, 2.5 % with e4m3).  The sums therefore leave tensor memory for registers, which hold them in
+// float32, every 16 tiles, and when a weight would exceed 2^4; the accumulation then starts anew with the largest weight of the present tile as the
+// reference, be it higher or lower.  2048 keys are off by 2^-17 of 2^ref at most, a key among them weighs half of that or more: 2^-16 of the sum of the
+// weights, however many the keys.  References are whole numbers, so that the sums are scaled without roundings.  All waits are bounded.
 #include "att_sm100_common.cuh"
 #include "paged_decode.cuh"
 
@@ -29,7 +32,13 @@ constexpr int PT_THREADS = 6 * 32;
 constexpr int PT_SOFT_THREADS = PT_SOFT_WARPS * 32;
 constexpr int PT_KEYS = PD_RANGE_TILE;
 constexpr int PT_TMEM_COLS = 128;         // scores twice 16, result up to 64
-constexpr int PT_DRAIN_TILES = 1000;      // digits * codes stay below 2^14: 2^31 after 1024 tiles of 128 keys
+constexpr int PT_DRAIN_TILES = 16;        // int32 would overflow after 1024 (digits * codes up to 2^14)
+constexpr float PT_EDGE = 4.0f - 1.0f / 64; // log2 of the largest weight: the digits of int8 end at 2^4 * 0.996
+constexpr float PT_I8_UNIT = 1 << 27, PT_E4M3_UNIT = 16.0f; // what a weight of 1 is in digits
+constexpr float PT_E4M3_STEP = 32.0f;     // from a digit to the next: roundings of numbers up to 256 leave 8 at most, so that the next is up to 256 again
+// log2 of what a reference may lie below the range's highest: 2^30 keys of 2^(84 + 12) each can still be summed in float32, and of keys far below that
+// one 8 million are off by 2^-17 of it
+constexpr float PT_SINK = 12.0f;
 
 // what the weights need of a tile's keys besides their scores
 struct TTileKeys {
@@ -59,6 +68,7 @@ struct TTcMisc {
     int Fresh[2];                // the product with these weights starts a new sum
     alignas(16) float Mult[2][PD_ROWS];     // query scale times the logits' factor, of this unit and the next
     alignas(16) float Ref[PD_ROWS];
+    float Top[PD_ROWS];          // the highest reference so far
     float Red[PT_SOFT_WARPS][PD_ROWS];
     alignas(16) float Factor[PD_ROWS];
 };
@@ -80,14 +90,20 @@ __device__ __forceinline__ bool SoftAny(bool x)
     return r != 0;
 }
 
-// two weights' next e4m3 digits; a and b become 16 times what is left over
+// two weights' next e4m3 digits; a and b become PT_E4M3_STEP times what is left over
 __device__ __forceinline__ uint32_t TakeDigit(float &a, float &b)
 {
     const uint32_t d = PackE4M3x2(a, b);
     const float2 f = UnpackE4M3x2(d);
-    a = (a - f.x) * 16.0f;
-    b = (b - f.y) * 16.0f;
+    a = (a - f.x) * PT_E4M3_STEP;
+    b = (b - f.y) * PT_E4M3_STEP;
     return d;
+}
+
+// 2^n of a whole number up to 127, without a rounding; 0 below 2^-126
+__device__ __forceinline__ float WholeExp2(float n)
+{
+    return n < -126.0f ? 0.0f : __int_as_float(((int)n + 127) << 23);
 }
 
 // floats as integers of the same order
@@ -433,7 +449,7 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
             const int firstHead = head * p.Group + chunk * PD_ROWS, rows = min(p.Group - chunk * PD_ROWS, PD_ROWS);
             more = walk.Next(p, seg);
             if (tid < PD_ROWS) {
-                misc.Ref[tid] = PD_NO_REF;
+                misc.Ref[tid] = misc.Top[tid] = PD_NO_REF;
             }
             float sum[HEADS], acc[HEADS];
 #pragma unroll
@@ -452,10 +468,12 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         if (E4M3) { // column 4 k + h: digit k
-                            acc[4 * b + h] += __uint_as_float(r[h]) + 0.0625f * (__uint_as_float(r[4 + h]) + 0.0625f * (__uint_as_float(r[8 + h]) + 0.0625f * __uint_as_float(r[12 + h])));
+                            constexpr float STEP = 1 / PT_E4M3_STEP;
+                            const float x = fmaf(STEP, fmaf(STEP, fmaf(STEP, __uint_as_float(r[12 + h]), __uint_as_float(r[8 + h])), __uint_as_float(r[4 + h])), __uint_as_float(r[h]));
+                            acc[4 * b + h] = fmaf(x, 1 / PT_E4M3_UNIT, acc[4 * b + h]);
                         } else { // column 4 h + k: digit k, the lowest first
                             const float lo = fmaf(256.0f, (float)(int)r[4 * h + 1], (float)(int)r[4 * h]), hi = fmaf(256.0f, (float)(int)r[4 * h + 3], (float)(int)r[4 * h + 2]);
-                            acc[4 * b + h] = fmaf(fmaf(65536.0f, hi, lo), 1.0f / (1 << 22), acc[4 * b + h]);
+                            acc[4 * b + h] = fmaf(fmaf(65536.0f, hi, lo), 1 / PT_I8_UNIT, acc[4 * b + h]);
                         }
                     }
                 }
@@ -476,7 +494,7 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
                 }
                 const float ks = tileKeys[stage].KScale[tid], vs = tileKeys[stage].VScale[tid], bias = tileKeys[stage].Bias[tid];
                 const bool valid = bias < INFINITY || bias != bias;
-                const float edge = ReferenceEdge(vs);
+                const float edge = ReferenceEdge(vs, PT_EDGE);
                 if (!dead && !WaitBarA<true>(&misc.SReady[buf], (count / 2) & 1, abortFlag)) {
                     dead = true;
                     fail(kDevTimeoutMma);
@@ -525,14 +543,10 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
                 }
                 bool fresh = sinceDrain == 0;
                 if (SoftAny(raise || dead || sinceDrain >= PT_DRAIN_TILES)) {
-                    if (sinceDrain > 0 && !dead && !lastProduct(count - 1)) {
-                        dead = true;
-                        fail(kDevTimeoutMma);
-                    }
-                    // new references: the largest z + log2 vScale of the tile's keys
+                    // new references: the largest z + log2 |vScale| of the tile's keys, not far below the highest so far; a tile without keys leaves them
 #pragma unroll
                     for (int h = 0; h < HEADS; ++h) {
-                        const int m = __reduce_max_sync(0xffffffffu, OrderedInt(z[h] != z[h] ? -INFINITY : z[h] - edge + 8.0f));
+                        const int m = __reduce_max_sync(0xffffffffu, OrderedInt(z[h] != z[h] ? -INFINITY : z[h] - edge + PT_EDGE));
                         if (lane == 0) {
                             misc.Red[warp][h] = FromOrderedInt(m);
                         }
@@ -541,14 +555,22 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
                         break;
                     }
                     if (sinceDrain > 0) {
+                        if (!lastProduct(count - 1)) {
+                            dead = true;
+                            fail(kDevTimeoutMma);
+                        }
+                        __syncwarp();
                         drain();
                     }
                     float old = 0, ref = 0;
                     if (tid < HEADS) {
                         old = misc.Ref[tid];
-                        ref = fmaxf(fmaxf(old, fmaxf(misc.Red[0][tid], misc.Red[1][tid])), fmaxf(misc.Red[2][tid], misc.Red[3][tid]));
+                        const float most = ceilf(fmaxf(fmaxf(misc.Red[0][tid], misc.Red[1][tid]), fmaxf(misc.Red[2][tid], misc.Red[3][tid])));
+                        const float top = fmaxf(misc.Top[tid], most);
+                        ref = most == -INFINITY ? old : fmaxf(most, top - PT_SINK);
+                        misc.Top[tid] = top;
                         misc.Ref[tid] = ref;
-                        misc.Factor[tid] = Exp2(old - ref);
+                        misc.Factor[tid] = WholeExp2(old - ref);
                     }
                     SoftAny(false);
 #pragma unroll
@@ -572,9 +594,10 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
                     }
                     uint4 x;
                     if (E4M3) {
+                        const float scale = vs * PT_E4M3_UNIT;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            w[i] *= vs;
+                            w[i] *= scale;
                         }
                         uint32_t d[4];
 #pragma unroll
@@ -585,7 +608,7 @@ __global__ void __launch_bounds__(PT_THREADS, (TTcLayout<D, HB>::CTAS)) PagedRan
                         x = make_uint4(d[0], d[1], d[2], d[3]);
                     } else {
                         uint32_t d[4];
-                        const float scale = vs * (float)(1 << 22);
+                        const float scale = vs * PT_I8_UNIT;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             d[i] = ((uint32_t)__float2int_rn(w[i] * scale) + 0x80808080u) ^ 0x80808080u; // signed digits of base 256
