@@ -406,8 +406,9 @@ size_t tsa_paged_decode_workspace_bytes(const tsa_paged_cfg *cfg, const tsa_page
  *   moves      int32 [nSeq][kv_heads][moveCap][2]  (slot to write, slot to read), the rest (-1, -1)
  *   moveCounts int32 [nSeq][kv_heads]
  *   newLens    int32 [nSeq]                        min(ctxLens[s], keep)
- * all device memory; moveCap at least min(keep, maxCtx - keep) and 1.  Sequences of up to `keep` slots have no moves.  Needs weight;
- * of the cache only pos and weight are read (k, v and the scales may be NULL).  keep >= 1, 0 <= recent <= keep. */
+ * all device memory that overlaps neither ctxLens nor tokens; moveCap at least min(keep, maxCtx - keep) and 1.  Sequences of up to `keep`
+ * slots have no moves.  Needs weight; of the cache only pos and weight are read (k, v and the scales may be NULL).  keep >= 1,
+ * 0 <= recent <= keep. */
 int tsa_paged_evict_select(const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens, int nSeq, int maxCtx, int keep,
     int recent, int *moves, int moveCap, int *moveCounts, int *newLens, int *statusWord, tsa_stream_t stream);
 

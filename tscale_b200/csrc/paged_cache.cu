@@ -830,6 +830,11 @@ __global__ void __launch_bounds__(MOV_WARPS * 32) PagedMoveKernel(const TMovePar
     }
 }
 
+static bool Overlap(const void *a, size_t aBytes, const void *b, size_t bBytes)
+{
+    return a && b && (uintptr_t)a < (uintptr_t)b + bBytes && (uintptr_t)b < (uintptr_t)a + aBytes;
+}
+
 } // namespace tsa
 
 using namespace tsa;
@@ -902,6 +907,12 @@ extern "C" __attribute__((visibility("default"))) int tsa_paged_evict_select(con
     TSA_REQUIRE(moves && moveCounts && newLens, "tsa_paged_evict_select: null moves/moveCounts/newLens");
     TSA_REQUIRE(moveCap >= 1 && moveCap >= most, "tsa_paged_evict_select: room for %d moves of a head needed, %d given", most < 1 ? 1 : most, moveCap);
     TSA_REQUIRE((uintptr_t)moves % 8 == 0, "tsa_paged_evict_select: moves must be 8-byte aligned");
+    // a CTA of one key head may write its part before another has read the lengths
+    const size_t counts = (size_t)nSeq * kv->kv_heads * sizeof(int), lens = (size_t)nSeq * sizeof(int);
+    for (const int *in : {ctxLens, tokens}) {
+        TSA_REQUIRE(!Overlap(newLens, lens, in, lens) && !Overlap(moveCounts, counts, in, lens) && !Overlap(moves, counts * moveCap * 2, in, lens),
+            "tsa_paged_evict_select: moves, moveCounts and newLens must not overlap ctxLens or tokens");
+    }
     p.CtxLens = ctxLens;
     p.Tokens = tokens;
     p.NSeq = nSeq;
