@@ -524,6 +524,13 @@ const at::Tensor *IntVector(PyObject *o, int64_t n)
     return t;
 }
 
+const at::Tensor *StatusWord(PyObject *o)
+{
+    const at::Tensor *t = Tensor(o);
+    Need(!t || (t->scalar_type() == at::kInt && t->numel() >= 1), PyExc_AssertionError, "expected an int32 status word");
+    return t;
+}
+
 // two-dimensional argument of a 32-bit type
 tsa_ptr2d Plane(const at::Tensor *t, at::ScalarType type, const char *text)
 {
@@ -600,7 +607,7 @@ PyObject *PagedAppend(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return Guard<10>(n, [&] {
         const TPaged p(a[0], a[1], a[2], a[3], true);
-        const at::Tensor *starts = IntVector(a[4], p.NSeq + 1), *status = Tensor(a[9]);
+        const at::Tensor *starts = IntVector(a[4], p.NSeq + 1), *status = StatusWord(a[9]);
         const at::Tensor &k = NeedTensor(a[5]), &ks = NeedTensor(a[6]), &v = NeedTensor(a[7]), &vs = NeedTensor(a[8]);
         const tsa_ptr2d k2 = p.Codes(k), v2 = p.Codes(v), ks2 = Plane(&ks, at::kFloat, "expected float32 scales of the new rows"),
                         vs2 = Plane(&vs, at::kFloat, "expected float32 scales of the new rows");
@@ -620,7 +627,7 @@ PyObject *PagedDecode(PyObject *, PyObject *const *a, Py_ssize_t n)
     return Guard<14>(n, [&] {
         TPaged p(a[0], a[1], a[2], a[3], true);
         const at::Tensor &q = NeedTensor(a[5]);
-        const at::Tensor *qs = Tensor(a[6]), *given = Tensor(a[11]), *ws = Tensor(a[12]), *status = Tensor(a[13]);
+        const at::Tensor *qs = Tensor(a[6]), *given = Tensor(a[11]), *ws = Tensor(a[12]), *status = StatusWord(a[13]);
         const tsa_ptr2d q2 = p.Codes(q), qs2 = Plane(qs, at::kFloat, "expected float32 query scales");
         Need(p.Cfg.head_dim > 0 && q2.xsize % p.Cfg.head_dim == 0, PyExc_AssertionError, "expected queries [sequences][heads * head size]");
         const int heads = q2.xsize / p.Cfg.head_dim, window = Int32(a[8]);
@@ -649,7 +656,7 @@ PyObject *PagedEvictSelect(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return Guard<8>(n, [&] {
         const TPaged p(a[0], a[1], a[2], a[3], false);
-        const at::Tensor *status = Tensor(a[7]);
+        const at::Tensor *status = StatusWord(a[7]);
         const int maxCtx = a[4] == Py_None ? Size((int64_t)p.Table.xsize * p.Kv.page_size) : Int32(a[4]), keep = Int32(a[5]), recent = Int32(a[6]);
         p.OneGpu({status});
         const c10::cuda::CUDAGuard guard(p.First().device());
@@ -669,7 +676,7 @@ PyObject *PagedEvictSelect(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyObject *PagedEvictMove(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return Guard<5>(n, [&] {
-        const at::Tensor &moves = NeedTensor(a[2]), *status = Tensor(a[4]);
+        const at::Tensor &moves = NeedTensor(a[2]), *status = StatusWord(a[4]);
         const TPaged p(a[0], a[1], a[3], Py_None, true); // the counts in the place of the lengths
         Need(moves.dim() == 4 && moves.scalar_type() == at::kInt && moves.is_contiguous() && moves.size(3) == 2 && moves.size(1) == p.Kv.kv_heads && p.Lens->dim() == 2 &&
                 p.Lens->size(0) == moves.size(0) && p.Lens->size(1) == moves.size(1),
