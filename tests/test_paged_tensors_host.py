@@ -21,3 +21,11 @@ CALLS = [lambda **kw: ops.paged_append(KV, TABLE, CTX, ROW, SCALE, ROW, SCALE, t
 def test_status_words(call, status, text):
     with pytest.raises(AssertionError, match=text):
         call(status=status)
+
+
+@pytest.mark.parametrize("workspace,text", [(torch.zeros(1, dtype=torch.uint8).expand(1 << 20), "contiguous"), (torch.zeros(1 << 12, dtype=torch.uint8)[::2], "contiguous"),
+                                            (torch.zeros((64, 64)).t(), "contiguous"), (torch.zeros(1 << 12, dtype=torch.uint8), "one GPU")])
+def test_workspaces(workspace, text):
+    """Memory that a tensor only seems to have, or that lies between its elements."""
+    with pytest.raises(AssertionError, match=text):
+        CALLS[1](workspace=workspace)

@@ -635,6 +635,7 @@ PyObject *PagedDecode(PyObject *, PyObject *const *a, Py_ssize_t n)
         const float slope = Float(a[9]);
         p.Cfg.qk_vec_scale = Float(a[7]);
         p.Cfg.out_dtype = given ? TsaType(*given) : (int)Int(a[10]);
+        Need(!ws || ws->is_contiguous(), PyExc_AssertionError, "expected a contiguous workspace"); // it counts with nbytes()
         p.OneGpu({&q, qs, given, ws, status});
         const c10::cuda::CUDAGuard guard(p.First().device());
         const at::Tensor out = given ? *given : Empty(p.NSeq, (int64_t)heads * p.Cfg.head_dim, TorchType(p.Cfg.out_dtype), q);
