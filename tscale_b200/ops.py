@@ -430,7 +430,8 @@ class PagedKVCache:
 
     def extend(self, counts=1):
         """Makes room for counts[s] new tokens of each sequence (one number: the same for all), which the next `append` stores.  Returns the
-        row_starts of that append; None where every sequence gets one row.  Raises TsaError, and changes nothing, if the pages do not suffice."""
+        row_starts of that append; None where every sequence gets one row.  Raises TsaError, and changes nothing, if the pages do not suffice or a
+        sequence has seen more than 2^31 - 1 tokens."""
         counts = np.broadcast_to(np.asarray(counts, dtype=np.int64), (self.n_seq,))
         if (counts < 0).any():
             raise abi.TsaError(abi.TSA_BAD_ARG, "PagedKVCache.extend: negative count")
@@ -439,6 +440,8 @@ class PagedKVCache:
         if after.max() > self.max_pages or need.sum() > len(self.free):
             raise abi.TsaError(abi.TSA_BAD_ARG, "PagedKVCache.extend: %d pages needed, %d free; a sequence has at most %d"
                                % (need.sum(), len(self.free), self.max_pages))
+        if (self.seen + counts).max() > 0x7fffffff:
+            raise abi.TsaError(abi.TSA_BAD_ARG, "PagedKVCache.extend: a sequence's positions end at 2^31 - 2")
         for s in np.flatnonzero(need):
             for i in range(have[s], after[s]):
                 self._table[s, i] = self.free.pop()
