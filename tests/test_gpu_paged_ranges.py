@@ -10,7 +10,7 @@ import ctypes
 import pytest
 import torch
 
-from tests.test_gpu_paged import CODES, DEV, DOT, WHOLE, _gen
+from tests.test_gpu_paged import CODES, DEV, DOT, ERR, MANY, WHOLE, Cache, _check_out, _codes, _decode_ref, _gen, _query, _unit
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +64,225 @@ def test_one_heavy_key_among_very_many_light_ones(kv, d, group, logits):
     tol = 2.0 ** -16 * float(values.abs().max()) + 2.0 ** -15 * (w @ values.abs())
     off = (got.double().view(n_seq, group, d) - (w @ values)).abs()
     assert not (off > tol).any(), float((off / tol).max())
+
+
+LENS = MANY * 3 + [520, 385]  # with sixteen key heads: more units than there are clusters of any kind for
+
+
+@pytest.mark.parametrize("kv,scale,d,heads,kvh,page,window,slope,out,track", [
+    ("i8", torch.float16, 128, 16, 16, 64, WHOLE, 0.0, torch.float32, False),
+    ("e4m3", torch.float16, 128, 64, 16, 16, WHOLE, 0.01, torch.bfloat16, False),
+    ("i8", torch.float32, 128, 96, 16, 32, 600, 0.0, torch.float32, True),      # six query heads per key head
+    ("e4m3", torch.float32, 128, 144, 16, 128, WHOLE, 0.02, torch.float32, True),  # nine
+    ("e4m3", torch.float16, 128, 256, 16, 32, 600, 0.0, torch.float16, False),  # sixteen
+    ("i8", torch.float32, 128, 208, 16, 256, 600, 0.01, torch.float32, True),
+    ("i8", torch.float16, 64, 16, 16, 32, WHOLE, 0.01, torch.float32, True),
+    ("e4m3", torch.float32, 64, 80, 16, 16, WHOLE, 0.0, torch.float32, False),
+    ("i8", torch.float16, 64, 288, 16, 64, 600, 0.0, torch.bfloat16, True),     # eighteen: two units
+    ("e4m3", torch.float16, 64, 192, 16, 256, WHOLE, 0.0, torch.float32, True),
+])
+def test_many_units(kv, scale, d, heads, kvh, page, window, slope, out, track):
+    from tscale_b200 import ops
+    c = Cache(31, LENS, kvh, d, page, kv, scale, track)
+    q, qs = _query(31, len(LENS), heads, d, kv)
+    before = None if c.weight is None else c.weight.clone()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    want, added = _decode_ref(c, q, qs, heads, window, slope)
+    _needs_workspace(c.kv, len(LENS), heads, max(LENS), window)
+    got = ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, slope, max_ctx=max(LENS), out_dtype=out, tokens=c.tokens, status=status)
+    assert int(status) == 0 and not got[0].any()
+    _check_out(got, want, c)
+    if track:
+        for (s, h), w in added.items():
+            p, o = c.place(s)
+            assert float((c.weight[p, h, o].double() - before[p, h, o].double() - w).abs().max()) <= ERR * (heads // kvh) + 2.0 ** -23
+            assert (c.weight[p, h, o][w == 0] == before[p, h, o][w == 0]).all()
+        assert c.weight[~c.live].isnan().all()
+    else:
+        assert torch.equal(got, ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, slope, max_ctx=max(LENS), out_dtype=out, tokens=c.tokens))
+
+
+@pytest.mark.parametrize("lens,d,heads,kvh", [(LENS, 128, 16, 16), (LENS, 128, 128, 16), (LENS, 128, 208, 16), (LENS, 64, 32, 16), (LENS, 64, 160, 16),
+                                              ([9000, 4500], 128, 4, 1), ([9000, 4500], 64, 14, 1)])
+@pytest.mark.parametrize("kv", ["i8", "e4m3"])
+@pytest.mark.parametrize("down", [False, True])
+def test_logits_that_rise_or_fall(lens, d, heads, kvh, kv, down):
+    """By 60 powers of two along the cache: references move in nearly every tile one way, and every sixteen tiles the other."""
+    from tscale_b200 import ops
+    c = Cache(32, lens, kvh, d, 32, kv, torch.float32, False)
+    one = 40 if kv == "i8" else 1
+    c.k.view(torch.int8).copy_(torch.full(c.k.shape, one, device=DEV).to(c.k.dtype).view(torch.int8))
+    q, qs = torch.full((len(lens), heads * d), one, device=DEV).to(CODES[kv]), torch.ones((len(lens), heads), device=DEV)
+    unit = one * one * d * DOT / d ** 0.5
+    for s, n in enumerate(lens):
+        line = torch.linspace(-30, 30, max(n, 2), device=DEV)[:n] / unit
+        for h in range(kvh):
+            c.write(c.ks, s, h, -line if down else line)
+    want, _ = _decode_ref(c, q, qs, heads, WHOLE, 0.0)
+    _needs_workspace(c.kv, len(lens), heads, max(lens))
+    _check_out(ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0, max_ctx=max(lens)), want, c)
+
+
+@pytest.mark.parametrize("kv,d,group", [("i8", 128, 2), ("e4m3", 128, 10), ("i8", 64, 12), ("e4m3", 64, 1)])
+def test_nan_and_infinity_stay_in_their_unit(kv, d, group):
+    from tscale_b200 import ops
+    kvh, seq, head = 16, 7, 5
+    c = Cache(33, LENS, kvh, d, 16, kv, torch.float16, False)
+    q, qs = _query(33, len(LENS), kvh * group, d, kv)
+    _needs_workspace(c.kv, len(LENS), kvh * group, max(LENS))
+    call = lambda window=WHOLE: ops.paged_decode(c.kv, c.table, c.ctx, q, qs, window, 0.0, max_ctx=max(LENS))  # noqa: E731
+    clean, part, cols = call(), call(800), slice(head * group * d, (head + 1) * group * d)
+    p, o = c.place(seq)  # 1000 tokens
+    assert c.lens[seq] == 1000
+    at = p[150], head, o[150]
+    for plane, x in ((c.ks, float("nan")), (c.vs, float("nan")), (c.vs, float("inf")), (c.ks, float("inf"))):
+        keep = plane[at].clone()
+        plane[at] = x
+        got = call()
+        assert got[seq, cols].isnan().all() or (plane is c.ks and x == float("inf"))  # a logit of minus infinity is none
+        got[seq, cols] = clean[seq, cols]
+        assert torch.equal(got, clean) and torch.equal(call(800), part)  # in front of the window: not attended
+        plane[at] = keep
+    if kv == "e4m3":
+        for plane in (c.k, c.v):
+            keep = plane.view(torch.uint8)[at].clone()
+            plane.view(torch.uint8)[at] = 0x7f
+            got = call()
+            assert got[seq, cols].isnan().all()
+            got[seq, cols] = clean[seq, cols]
+            assert torch.equal(got, clean) and torch.equal(call(800), part)
+            plane.view(torch.uint8)[at] = keep
+    assert torch.equal(call(), clean)
+
+
+@pytest.mark.parametrize("kv,d,group,track", [("i8", 128, 1, True), ("e4m3", 128, 12, False), ("i8", 64, 3, False), ("e4m3", 64, 9, True)])
+def test_pages_outside_the_pool_and_sequences_beyond_the_bound(kv, d, group, track):
+    from tscale_b200 import ops
+    kvh, seq = 16, 7
+    c = Cache(34, LENS, kvh, d, 16, kv, torch.float16, track)
+    q, qs = _query(34, len(LENS), kvh * group, d, kv)
+    _needs_workspace(c.kv, len(LENS), kvh * group, 600)
+    start = None if c.weight is None else c.weight.clone()
+
+    def call(table=c.table, **kw):
+        if track:
+            c.weight.copy_(start)
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        return ops.paged_decode(c.kv, table, c.ctx, q, qs, WHOLE, 0.0, tokens=c.tokens, status=status, **kw), int(status)
+
+    clean, status = call(max_ctx=1000)
+    after = None if c.weight is None else c.weight.clone()
+    assert status == 0
+    p, o = c.place(seq)
+    others = [s for s in range(len(LENS)) if s != seq]
+    for bad in (-1, c.k.shape[0], 0x7fffffff, -0x80000000):
+        table = c.table.clone()
+        table[seq, 3] = bad
+        got, status = call(table, max_ctx=1000)
+        assert status != 0 and got.isfinite().all() and torch.equal(got[others], clean[others])
+        if track:  # the page's slots keep their weights, other sequences get theirs
+            assert torch.equal(c.weight[p[48:64], :, o[48:64]], start[p[48:64], :, o[48:64]])
+            for s in others:
+                ps, os = c.place(s)
+                assert torch.equal(c.weight[ps, :, os], after[ps, :, os])
+    # sequences beyond the bound, and beyond their row of the table
+    long = [s for s, n in enumerate(LENS) if n > 650]
+    rest = [s for s, n in enumerate(LENS) if n <= 650]
+    limit = 2 * ERR * float((c.v.float().nan_to_num() * c.vs.float().nan_to_num()[..., None]).abs().max())
+    for table, bound in ((c.table, 650), (c.table[:, :41], 1000)):
+        got, status = call(table, max_ctx=bound)
+        assert status != 0 and not got[long].any() and float((got[rest] - clean[rest]).abs().max()) <= limit
+        if track:
+            for s in long:
+                ps, os = c.place(s)
+                assert torch.equal(c.weight[ps, :, os], start[ps, :, os])
+
+
+@pytest.mark.parametrize("kv,d,group,track", [("i8", 128, 2, True), ("e4m3", 128, 16, False), ("i8", 64, 1, True), ("e4m3", 64, 8, False), ("i8", 64, 16, True)])
+def test_calls_in_a_row_share_a_workspace(kv, d, group, track):
+    """A workspace of just the size that is asked for, calls that follow one another without a wait, and lengths that a kernel between them changes."""
+    from tscale_b200 import abi, ops
+    kvh = 16
+    c = Cache(35, LENS, kvh, d, 64, kv, torch.float16, track)
+    q, qs = _query(35, len(LENS), kvh * group, d, kv)
+    size = _needs_workspace(c.kv, len(LENS), kvh * group, 1000)
+    space = torch.full((size + 4096,), 0xa5, dtype=torch.uint8, device=DEV)
+    cuts = [0, 300, 40, 700, 1, 129]
+    start = None if c.weight is None else c.weight.nan_to_num(0.0).clone()
+
+    def calls(**kw):
+        if track:
+            c.weight.copy_(start)
+        ctx, tokens, outs = c.ctx.clone(), None if c.tokens is None else c.tokens.clone(), []
+        for i, cut in enumerate(cuts):
+            torch.sub(c.ctx, cut, out=ctx).clamp_(min=0)
+            outs.append(ops.paged_decode(c.kv, c.table, ctx, q if i % 2 else q.flip(0), qs, WHOLE, 0.0, max_ctx=1000, tokens=tokens, **kw))
+        return outs + ([c.weight.clone()] if track else [])
+
+    want = []
+    for own in (True, False):
+        got = calls(**(dict(workspace=space[:size]) if own else {}))
+        torch.cuda.synchronize()
+        want.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*want)) and (space[size:] == 0xa5).all()
+    # one call alone, of the last lengths
+    if not track:
+        torch.cuda.synchronize()
+        alone = ops.paged_decode(c.kv, c.table, (c.ctx - cuts[3]).clamp(min=0), q, qs, WHOLE, 0.0, max_ctx=1000)
+        torch.cuda.synchronize()
+        assert torch.equal(alone, want[0][3])
+    with pytest.raises(abi.TsaError, match="workspace"):
+        ops.paged_decode(c.kv, c.table, c.ctx, q, qs, WHOLE, 0.0, max_ctx=1000, tokens=c.tokens, workspace=space[:size - 1])
+
+
+@pytest.mark.parametrize("kv,d,group,evict", [("i8", 128, 1, True), ("e4m3", 128, 12, False), ("i8", 64, 2, True), ("e4m3", 64, 1, False)])
+def test_captured_calls_and_streams(kv, d, group, evict):
+    """Appends and decodes of a cache as two graphs that are replayed in turn, beside a second cache that is called; then two streams at once."""
+    from tscale_b200 import ops
+    kvh, n_seq, most = 16, 38, 1000
+    heads, gen = kvh * group, _gen(36)
+    caches = [ops.PagedKVCache(n_seq, n_seq * 63, kvh, d, DEV, page_size=16, max_pages=63, kv_dtype=kv, evict=evict) for _ in range(2)]
+    _needs_workspace(caches[0].kv, n_seq, heads, most)
+    new = lambda rows: tuple(x for _ in range(2) for x in (_codes((rows, kvh * d), kv, gen), (torch.rand((kvh, rows), generator=gen, device=DEV) + 0.5) * _unit(kv)))  # noqa: E731
+    counts = [(s * 211) % 950 for s in range(n_seq)]
+    prompt, step = new(sum(counts)), new(n_seq)
+    q, qs = _query(36, n_seq, heads, d, kv)
+    for cache in caches:
+        cache.append(*prompt, cache.extend(counts))
+        cache.extend()
+    replayed, called = caches
+    side, graphs = torch.cuda.Stream(), []
+    keep = None if not evict else replayed.kv.weight.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                replayed.append(*step)
+                out = replayed.decode(q, qs, WHOLE, 0.0, max_ctx=most)
+            graphs.append((graph, out))
+    torch.cuda.current_stream().wait_stream(side)
+    assert keep is None or torch.equal(keep, replayed.kv.weight)
+    for i in range(8):
+        if i:
+            for cache in caches:
+                cache.extend()
+            for x in (*step, q):
+                x.copy_(x.view(torch.int8).flip(0).view(x.dtype) if x.element_size() == 1 else x.flip(0))
+        graph, out = graphs[i % 2]
+        graph.replay()
+        called.append(*step)
+        want = called.decode(q, qs, WHOLE, 0.0, max_ctx=most)
+        assert torch.equal(out, want) and out.isfinite().all() and out.any(), i
+        assert not evict or torch.equal(replayed.kv.weight, called.kv.weight), i
+    if evict:
+        return  # calls that add weights are ordered by one stream
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    other = q.view(torch.int8).flip(0).view(q.dtype).contiguous()
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(called.decode(other if i % 2 else q, qs, WHOLE, 0.0, max_ctx=most))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, outs[i % 2]) for i, x in enumerate(outs)) and not torch.equal(outs[0], outs[1]) and torch.equal(outs[0], want)
