@@ -38,3 +38,30 @@ def test_rows_without_a_place(kv, scale, kvh, d, track, ctx, pages):
     status = torch.zeros(1, dtype=torch.int32, device=DEV)
     ops.paged_append(c.kv, table.to(DEV), torch.tensor(ctx, dtype=torch.int32, device=DEV), k, ks, v, vs, torch.tensor(starts, dtype=torch.int32, device=DEV), c.tokens, status)
     assert int(status) != 0 and all(_same(a, b) for a, b in zip(planes, want))
+
+
+@pytest.mark.parametrize("kvh,d,rows", [(2, 64, 3000), (16, 128, 500)])
+def test_rows_that_the_kernel_before_writes(kvh, d, rows):
+    """The quantiser lets the next kernel start while it still writes; replayed, it writes other rows over those of the replay before."""
+    from tscale_b200 import ops
+    c = Cache(41, [rows], kvh, d, 64, "i8", torch.float32, False)
+    gen = _gen(41)
+    x, starts = torch.zeros((rows, kvh * d), device=DEV), torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    p, o = c.place(0)
+
+    def step():
+        k, ks = ops.quant_rows(x, "rms", "i8", d, vec_scale=1 / 24.0)
+        ops.paged_append(c.kv, c.table, c.ctx, k.view(torch.int8), ks, k.view(torch.int8), ks, starts)
+        return k, ks
+
+    x.copy_(torch.randn(x.shape, generator=gen, device=DEV))
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        k, ks = step()
+    for _ in range(20):
+        x.copy_(torch.randn(x.shape, generator=gen, device=DEV))
+        graph.replay()
+        for plane in (c.k, c.v):
+            assert torch.equal(plane[p, :, o].reshape(rows, -1), k.view(torch.int8))
+        assert torch.equal(c.ks[p, :, o], ks.t()) and torch.equal(c.vs[p, :, o], ks.t()) and k.any()

@@ -109,8 +109,8 @@ __global__ void __launch_bounds__(APP_WARPS * 32) PagedAppendKernel(const TAppen
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             if (i + j * lanes < pieces) {
-                a[j] = __ldg(ks + i + j * lanes);
-                b[j] = __ldg(vs + i + j * lanes);
+                a[j] = ks[i + j * lanes]; // not through the read-only path: the kernel before may still write the rows when this one starts
+                b[j] = vs[i + j * lanes];
             }
         }
     };
