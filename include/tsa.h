@@ -381,7 +381,8 @@ typedef struct {
  * (the planes that tsa_norm_rope_quant and tsa_matmul_norm_rope_quant write), rounded to the nearest scale_dtype.  Rows
  * [rowStarts[s], rowStarts[s + 1]) (device int32 [nSeq + 1], ascending; NULL: one row per sequence) are sequence s's; ctxLens and
  * tokens count them already, so the last of them goes to slot ctxLens[s] - 1 with position tokens[s] - 1.  Rows in front of
- * rowStarts[0] or from rowStarts[nSeq] on are ignored.  Weights of the new slots become 0. */
+ * rowStarts[0] or from rowStarts[nSeq] on are ignored.  Weights of the new slots become 0: only tsa_paged_decode adds to them, so that
+ * an eviction right behind a prompt knows nothing of the attention inside the prompt, and keeps its newest tokens and its lowest slots. */
 int tsa_paged_append(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens,
     const int *rowStarts, int nSeq, int rows, tsa_ptr2d kNew, tsa_ptr2d kScaleNew, tsa_ptr2d vNew, tsa_ptr2d vScaleNew, int *statusWord,
     tsa_stream_t stream);
@@ -391,8 +392,11 @@ int tsa_paged_append(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d
  * h reads key head h / (headCount / kv_heads).  q 8-bit [nSeq][headCount * D] of kv_dtype, qScale f32 [nSeq][headCount] (may be
  * absent), out [nSeq][headCount * D] of out_dtype.  Sequences without keys give zeros.
  * A cache that keeps weights gets each attended key's weight, summed over the query heads of the key head, added to weight.
- * maxCtx: host-side upper bound of ctxLens; it sizes the launch, and a sequence that turns out longer gives zeros and a bit of the
- * status word.  Value scales below 2^-80 may count as zero.  The same call gives the same bits every time.
+ * maxCtx: host-side upper bound of ctxLens; it sizes the launch and the workspace (with weights: 4 bytes for each sequence, query head
+ * and slot up to it), so that a bound far above the lengths costs time and memory; a sequence that turns out longer gives zeros and a
+ * bit of the status word.  Value scales below 2^-80 may count as zero; those above 2^100 are out of range.  With logits up to 32 a
+ * result is off by less than 2^-14 of the largest value (code times scale), besides the rounding to out_dtype, however many the keys.
+ * The same call gives the same bits every time.
  * workspace: tsa_paged_decode_workspace_bytes(...) bytes for the same arguments (0: none needed), 16-byte aligned, not shared by calls in
  * flight at the same time. */
 int tsa_paged_decode(const tsa_paged_cfg *cfg, const tsa_paged_kv *kv, tsa_ptr2d pageTable, const int *ctxLens, const int *tokens, int nSeq,

@@ -7,7 +7,7 @@
 // The stream of the cache bounds it: 2 D bytes of codes and two scales per key and key head, each read once; for short caches the latency
 // of what depends on one another does.  Two forms:
 //   clusters (here): a cluster of up to 8 CTAs has a unit (the up to 16 query heads that share a key head of a sequence) and joins its sums
-//     through distributed shared memory: one kernel, for caches of up to 4096 slots while all clusters are resident at once, and for windows of
+//     through distributed shared memory: one kernel, for caches of up to 4080 slots while all clusters are resident at once, and for windows of
 //     up to 1024 positions of longer caches with positions, whose keys it lists first.
 //   ranges (paged_decode_sm100.cu): all keys of all units, in a row, are cut into equal ranges, one for each CTA that can be resident; a
 //     unit that a range border cuts leaves partial sums, which a second kernel joins in the order of the ranges.
@@ -964,7 +964,9 @@ static TPagedForm PagedForm(int headDim, int nSeq, int kvHeads, int headCount, i
     //   units x slots   4 x 8192         32 x 4096         128 x 8192        512 x 3000         1024 x 8192      32 x 400000
     //   with            7.2 / 9.5        7.9 / 10.9        9.7 / 17.0        12.4 / 36.7        34 / 92          47 / 60
     //   without         11.5 / 11.6      14.0 / 14.0       42.8 / 42.6       62.6 / 62.5        278 / 278        401 / 401
-    // 512 slots to a CTA (1024: 4 units of 1500 slots, window 250, 9.2 instead of 8.1), as far as eight CTAs go.
+    // 512 slots to a CTA (1024: 4 units of 1500 slots, window 250, 9.2 instead of 8.1), as far as eight CTAs go.  (resident() counts four or three CTAs
+    // to an SM here too, where list and logits may leave place for fewer: sixteen heads x 128 with weights, window 1000, take 112 KB, so that 296 units of 4096
+    // slots take 42 us and 304 76.)
     w.ListCap = 0;
     const int listMax = window == 0 ? 1 : window;
     if (positions && listMax <= PD_MAX_LIST && maxCtx > PD_SPARSE_MIN && maxCtx / listMax >= (w.Cluster ? 4 : 2) && !(track && chunks > 1)) {

@@ -12,7 +12,7 @@
 // Measured: 64 sequences of 1024 .. 8192 slots, 16 key heads x 128 int8, 1.31 GB: 181 to 205 us, 6.4 to 7.2 TB/s (a plain copy: 6.45; mma.sync with
 // the codes in registers: 213 us); 48 of 500 .. 9000, 8 key heads x 128 e4m3 of four query heads, 0.5 GB: 84 to 94; 2 of 100000 .. 131072, 4 key heads of eight
 // query heads, 0.27 GB: 48.  What short calls lose is the start (lengths, page, first tile: 4 us) and the join; the tensor pipe is at 4 to 6 %, the
-// issue slots at 21 (four heads a unit) to 31 % (eight).
+// issue slots at 23 (128 dimensions, up to four heads a unit) to 41 % (64).
 //
 // One CTA: a warp that issues the copies (a box per page, up to 128 slots; tiles ahead of the arithmetic as far as the ring goes, across
 // units), one that issues the products, four for the weights.  Two CTAs per SM: while one of them ends a unit, the other has the memory.
